@@ -204,6 +204,51 @@ int mbrl_vjp_scan_sharded(const mbrl_model *m, int64_t B, int H, int grad_weight
 int mbrl_lane_map(int nq, int nv, int nu, int fd_mode, int *units_per_pair, int *unit, int *rollout, int *ref_lane,
                   int *primary);
 
+/* ---- optimiser-step operators over lists of tensors ----
+ * Between backward and the parameter update the reference bounds the gradient value by value and steps Adam one parameter at
+ * a time (model/blocks/policy/strategies.py:311-364, solver/build.py:4-25).  These work on the whole list at once: the
+ * global norm of all gradients, clipping by it, and the Adam update that takes the clipped gradient without writing it.
+ * A list is `count` tensors: host arrays of device pointers, numbers of values (0 is allowed, its pointer is not looked at) and
+ * element types (MBRL_DT_*; lists may mix them).  Each tensor is a dense run of values that starts at any element; the order
+ * of the values within it does not matter as long as a parameter, its gradient and its moments have the same.
+ * The host arrays are read before the call returns and not kept.  `workspace`: caller-owned device memory, 256-byte
+ * aligned, at least mbrl_optim_workspace_bytes(count) bytes, contents arbitrary before and after; one per call in flight
+ * (calls on the same stream may share one, captured graphs that can run at the same time must not).  All launches go to the
+ * calling thread's current HIP device, which must own the memory and the stream; no call waits for the device, and all can
+ * be captured into a HIP graph.  Results do not depend on timing: no atomics, every sum in a fixed order. */
+#define MBRL_DT_DOUBLE 0
+#define MBRL_DT_FLOAT 1
+#define MBRL_DT_BFLOAT 2
+#define MBRL_DT_HALF 3
+#define MBRL_NORM_INF 0        /* max |x| */
+#define MBRL_NORM_ONE 1        /* sum |x| */
+#define MBRL_NORM_TWO 2        /* sqrt(sum x^2) */
+int64_t mbrl_optim_workspace_bytes(int64_t count);
+
+/* norm[0] (device) = the norm over all values of all tensors, summed in fp64; 0 for an empty list; NaN if any value is.
+ * Squares of fp64 values beyond 1e154 overflow to an infinite norm. */
+int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel, const int *dtype, int norm_type,
+                   void *workspace, int64_t workspace_bytes, double *norm, void *hip_stream);
+
+/* The same, then every value is multiplied by min(1, max_norm / (norm + 1e-6)) in place (fp32 and fp64 in fp64, 16-bit types
+ * in fp32, rounded once).  A NaN norm makes every value NaN, an infinite one makes finite values 0 and infinite ones NaN.
+ * max_norm >= 0.  Tensors that share memory are refused (-7). */
+int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel, const int *dtype, int norm_type,
+                        double max_norm, void *workspace, int64_t workspace_bytes, double *norm, void *hip_stream);
+
+/* One Adam step of every tensor: with t = steps[i][0] + 1 (written back), g = c * grad (c the clipping factor above when
+ * `norm` is not NULL, else 1) and, unless `decoupled`, + weight_decay[i] * param,
+ *     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
+ *     param = param * (decoupled ? 1 - lr[i] weight_decay[i] : 1) - lr[i] / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps).
+ * exp_avgs (m) and exp_avg_sqs (v) are fp64 for fp64 parameters and fp32 for all others; gradients have their parameter's
+ * type and are left as they are.  Arithmetic in the moments' type, one rounding to a 16-bit parameter.  steps[i]: one
+ * fp32 value in device memory for each tensor.  norm != NULL: the norm over all gradients is left there (device).
+ * Memory that is written and shared with another tensor of the call is refused (-7). */
+int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads, void *const *exp_avgs,
+                   void *const *exp_avg_sqs, float *const *steps, const int64_t *numel, const int *dtype, const double *lr,
+                   const double *weight_decay, double beta_one, double beta_two, double eps, int decoupled, int norm_type,
+                   double max_norm, void *workspace, int64_t workspace_bytes, double *norm, void *hip_stream);
+
 const char *mbrl_last_error(void);
 
 #ifdef __cplusplus

@@ -1,14 +1,17 @@
-"""Build the HIP extension in-tree: csrc/models_gen.hpp (generated) + csrc/libmbrl_hip.so (hipcc, gfx950)."""
+"""Build the native code in-tree: csrc/models_gen.hpp (generated), csrc/libmbrl_hip.so (hipcc, gfx950) and
+csrc/optim_bind.so (g++: the argument lists of optim.py, which are Python lists of tensors)."""
 import os
 import shutil
 import subprocess
+import sysconfig
 
 from . import compile_planar
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libmbrl_hip.so")
-SOURCES = ["mbrl_hip.hip", "planar_lean.hpp", "wave_or.hpp", "models_gen.hpp"]
+BIND = os.path.join(CSRC, "optim_bind.so")
+SOURCES = ["mbrl_hip.hip", "planar_lean.hpp", "wave_or.hpp", "models_gen.hpp", "abi_error.hpp", "optim.hip"]
 
 
 def _hipcc():
@@ -34,7 +37,7 @@ def needs_build():
 # no-NaN / no-infinity / no-signed-zero arithmetic: lets x * 0.0 and x + 0.0 fold (model tables are full of zeros)
 # and drops the canonicalisation before min / max; non-finite results are still caught, by a test on the bits
 # (t_finite in planar_lean.hpp) that these flags cannot fold away.
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-pass-failed",
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-pass-failed",
                "-mllvm", "-pragma-unroll-threshold=1000000", "-mllvm", "-disable-machine-licm",
                "-mllvm", "-amdgpu-use-amdgpu-trackers=1",   # GCN register-pressure trackers in the scheduler: ~30 % fewer AGPR copies
                "-mllvm", "-amdgpu-sched-strategy=max-ilp",  # occupancy is pinned at one wave per SIMD anyway: schedule for
@@ -42,12 +45,42 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
                "-fno-honor-nans", "-fno-honor-infinities", "-fno-signed-zeros"]
 
 
+# The optimiser-step operators are a translation unit of their own: they promise IEEE results for infinities and NaN, which
+# the flags above give away, and gain nothing from that schedule.  No packed float32 instructions: some of their forms
+# have been seen to give wrong results.
+OPTIM_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def compile_lib(out, extra_flags=()):
-    """One hipcc line: csrc/mbrl_hip.hip -> `out` (also used by the profiling tools for their variants)."""
-    cmd = [_hipcc()] + HIPCC_FLAGS + list(extra_flags) + ["-o", out + ".tmp", os.path.join(CSRC, "mbrl_hip.hip")]
-    subprocess.check_call(cmd, cwd=CSRC)
+    """csrc/mbrl_hip.hip (with `extra_flags`: the profiling tools make their variants with it) and csrc/optim.hip -> `out`."""
+    objs = [out + ".main.o", out + ".optim.o"]
+    jobs = [subprocess.Popen([_hipcc()] + flags + ["-c", "-o", obj, os.path.join(CSRC, src)], cwd=CSRC)
+            for obj, src, flags in ((objs[0], "mbrl_hip.hip", HIPCC_FLAGS + list(extra_flags)), (objs[1], "optim.hip", OPTIM_FLAGS))]
+    if any([j.wait() for j in jobs]):
+        raise RuntimeError("hipcc failed")
+    subprocess.check_call([_hipcc(), "--offload-arch=gfx950", "-shared", "-o", out + ".tmp"] + objs, cwd=CSRC)
+    for obj in objs:
+        os.remove(obj)
     os.replace(out + ".tmp", out)
     return out
+
+
+def build_bind(force=False):
+    """csrc/optim_bind.cpp -> csrc/optim_bind.so: a CPython module over torch's C++ tensors (host code only)."""
+    src, deps = os.path.join(CSRC, "optim_bind.cpp"), [os.path.join(CSRC, "optim_bind.cpp"), os.path.join(HERE, "..", "include", "mbrl.h")]
+    if not force and os.path.exists(BIND) and all(os.path.getmtime(d) <= os.path.getmtime(BIND) for d in deps):
+        return BIND
+    import torch
+    from torch.utils import cpp_extension
+    rocm = os.path.dirname(os.path.dirname(_hipcc()))
+    inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(),
+           "-D__HIP_PLATFORM_AMD__=1"]        # the HIP runtime's headers ask a plain host compiler for it
+    cmd += ["-isystem" + d for d in inc] + ["-o", BIND + ".tmp", src, "-L" + libs, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
+    subprocess.check_call(cmd, cwd=CSRC)
+    os.replace(BIND + ".tmp", BIND)
+    return BIND
 
 
 def build_hip(force=False, verbose=False):

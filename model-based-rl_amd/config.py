@@ -85,7 +85,9 @@ _DEFAULTS = {
     "EXPERIENCE_REPLAY": {"SIZE": 2 ** 15, "SHUFFLE": True, "ENV_INIT_STATE_NUM": 2 ** 15 * 3 / 4},
     "SOLVER": {"OPTIMIZER": "adam", "BASE_LR": 0.001, "STD_LR_FACTOR": 0.001, "BIAS_LR_FACTOR": 2,
                "WEIGHT_DECAY_SD": 0.0, "MOMENTUM": 0.9, "WEIGHT_DECAY": 0.0005, "WEIGHT_DECAY_BIAS": 0,
-               "ADAM_BETAS": (0.9, 0.999)},
+               "ADAM_BETAS": (0.9, 0.999),
+               # additions of this build: bound of the global gradient norm (0: none), and Adam as one fused update (optim.py)
+               "CLIP_GRAD_NORM": 0.0, "FUSED": False},
     "OUTPUT": {"DIR": "./output", "NAME": "timestamp"},
     "LOG": {"PERIOD": 1, "PLOT": {"ENABLED": True, "DISPLAY_PORT": 8097, "ITER_PERIOD": 1},
             "TESTING": {"ENABLED": True, "ITER_PERIOD": 1, "RECORD_VIDEO": False, "COUNT_PER_ITER": 1},

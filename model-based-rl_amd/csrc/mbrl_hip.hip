@@ -24,6 +24,7 @@
 #include <new>
 
 #include "../../include/mbrl.h"
+#include "abi_error.hpp"
 
 #ifdef MBRL_PHASE_TIMING   // profiling build only (tools/phase_timing.py): shader-clock totals per solver phase
 // Light marks: the previous stamp lives in a scalar register pair, the per-wave totals in LDS (fire-and-forget
@@ -645,6 +646,7 @@ static int fail(int code, const char *fmt, const char *a = "", long long b = 0) 
     snprintf(g_err, sizeof g_err, fmt, a, b);
     return code;
 }
+int mbrl::report(int code, const char *text) { return fail(code, "%s", text); }
 
 // -DMBRL_ONLY_ENV=k (A/B and ISA-inspection builds): only model k is instantiated, the others report "unknown env"
 #ifdef MBRL_ONLY_ENV

@@ -16,7 +16,8 @@ EPISODE_MAJOR, TIME_MAJOR = 0, 1
 
 SYMBOLS = ("mbrl_abi_version", "mbrl_model_create", "mbrl_model_destroy", "mbrl_model_dims", "mbrl_step",
            "mbrl_fd_jacobians", "mbrl_fd_jacobians_closed_loop", "mbrl_fd_plan_bytes", "mbrl_fd_plan",
-           "mbrl_fd_jacobians_planned", "mbrl_fd_jacobians_static", "mbrl_step_record", "mbrl_rollout_record", "mbrl_fd_plan_finish", "mbrl_vjp_scan", "mbrl_vjp_scan_layout", "mbrl_vjp_scan_sharded", "mbrl_lane_map", "mbrl_last_error")
+           "mbrl_fd_jacobians_planned", "mbrl_fd_jacobians_static", "mbrl_step_record", "mbrl_rollout_record", "mbrl_fd_plan_finish", "mbrl_vjp_scan", "mbrl_vjp_scan_layout", "mbrl_vjp_scan_sharded", "mbrl_lane_map", "mbrl_last_error",
+           "mbrl_optim_workspace_bytes", "mbrl_grad_norm", "mbrl_clip_grad_norm", "mbrl_adam_step")
 
 _lib = None
 vp = C.c_void_p
@@ -59,6 +60,13 @@ def load():
     L.mbrl_step_record.argtypes = [vp, C.c_int64] + [vp] * 7 + [vp, C.c_int64, C.c_int64, C.c_int64, vp]
     L.mbrl_fd_plan_finish.argtypes = [vp, C.c_int64, vp, vp, C.c_int64, vp]
     L.mbrl_rollout_record.argtypes = [vp, C.c_int64, C.c_int] + [vp] * 5 + [vp, C.c_int64, C.c_int64, C.c_int64, vp]
+    ppv, pi64, pint, pf64 = C.POINTER(vp), C.POINTER(C.c_int64), C.POINTER(C.c_int), C.POINTER(C.c_double)
+    L.mbrl_optim_workspace_bytes.argtypes = [C.c_int64]
+    L.mbrl_optim_workspace_bytes.restype = C.c_int64
+    L.mbrl_grad_norm.argtypes = [C.c_int64, ppv, pi64, pint, C.c_int, vp, C.c_int64, vp, vp]
+    L.mbrl_clip_grad_norm.argtypes = [C.c_int64, ppv, pi64, pint, C.c_int, C.c_double, vp, C.c_int64, vp, vp]
+    L.mbrl_adam_step.argtypes = [C.c_int64, ppv, ppv, ppv, ppv, ppv, pi64, pint, pf64, pf64, C.c_double, C.c_double, C.c_double,
+                                 C.c_int, C.c_int, C.c_double, vp, C.c_int64, vp, vp]
     # test knobs outside include/mbrl.h (tests/test_gpu_overflow.py, tests/test_zz_no_alloc.py)
     L.mbrl_debug_set_flags.argtypes = [C.c_int]
     L.mbrl_debug_static_hold.argtypes = [vp, C.c_int, vp]

@@ -1,0 +1,160 @@
+"""Optimiser-step operators over lists of tensors on the HIP device: the global gradient norm, clipping by it, and the Adam
+update that takes the clipped gradient (C ABI: include/mbrl.h; kernels: csrc/optim.hip).
+
+The reference bounds gradients value by value and steps torch's Adam over its parameters
+(model/blocks/policy/strategies.py:311-364, solver/build.py:4-25).  Gradients that come through finite differences of contact
+dynamics can grow with every step of the horizon, and bounding their global norm keeps a direction that bounding values
+does not.  `strategies.VariationalOptimization.optimize` calls these under SOLVER.CLIP_GRAD_NORM and SOLVER.FUSED.
+
+All functions take lists of float64 / float32 / bfloat16 / float16 tensors of one GPU (types may be mixed), launch on the
+current stream, never wait for the device (but for error_if_nonfinite) and can be captured into a graph.  Tensors have to be
+dense -- any order of dimensions, any alignment, no gaps or repeats.  There is no CPU path.
+"""
+import ctypes as C
+import importlib.util
+import math
+import os
+
+import torch
+
+from . import lib
+
+_bind = None
+
+
+def bind():
+    """The host module that turns lists of tensors into the arguments of the C ABI (csrc/optim_bind.so)."""
+    global _bind
+    if _bind is None:
+        path = os.path.join(lib.HERE, "csrc", "optim_bind.so")
+        if not os.path.exists(path):
+            raise lib.MbrlError("host module not built: %s is missing (run __graft_entry__.build())" % path)
+        L = lib.load()
+        spec = importlib.util.spec_from_file_location("optim_bind", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.connect(lib.MbrlError, *(C.cast(getattr(L, n), C.c_void_p).value for n in
+                                   ("mbrl_optim_workspace_bytes", "mbrl_grad_norm", "mbrl_clip_grad_norm", "mbrl_adam_step",
+                                    "mbrl_last_error")))
+        _bind = m
+    return _bind
+
+
+def grad_norm(grads, norm_type=2.0):
+    """Norm over all values of all tensors in `grads` as a 0-d float64 tensor, summed in float64.  norm_type 1, 2 or inf.
+    0 for an empty list, NaN if any value is NaN."""
+    return (_bind or bind()).grad_norm(grads, norm_type)
+
+
+def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Multiplies every value of every tensor in `grads` by min(1, max_norm / (norm + 1e-6)), in place, and returns the norm
+    as it was (0-d float64).  A norm within the bound leaves the values untouched, bit for bit.  A NaN norm makes every
+    value NaN, an infinite one makes finite values 0; error_if_nonfinite=True raises RuntimeError before anything is
+    changed instead (it waits for the device, so not under graph capture).  Tensors that share memory are refused."""
+    b = _bind or bind()
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("clip_grad_norm_: error_if_nonfinite waits for the device and cannot be captured into a graph")
+        norm = float(b.grad_norm(grads, norm_type))
+        if not math.isfinite(norm):
+            raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % norm)
+    return b.clip_grad_norm_(grads, max_norm, norm_type)
+
+
+def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False,
+              max_norm=None, norm_type=2.0):
+    """One Adam step (torch.optim.Adam's arithmetic) of all `params`, in place, in as few launches as the list allows.
+
+    exp_avgs / exp_avg_sqs: float64 for float64 parameters, float32 for all others, shaped and laid out like their
+    parameter; steps: one float32 value in device memory each, counted up here; lr, weight_decay: one number or one for
+    each tensor; decoupled: weight decay on the parameter (AdamW) instead of on the gradient.  max_norm: the gradients enter
+    as clip_grad_norm_ would leave them, but are not written; returns their norm (0-d float64) then, else None.
+    Memory that is written must not be shared between tensors."""
+    return (_bind or bind()).adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay,
+                                       decoupled, max_norm, norm_type)
+
+
+class FusedAdam(torch.optim.Optimizer):
+    """torch.optim.Adam's rule as one adam_step over all parameters that have a gradient, with the gradients clipped by their
+    global norm on the way (max_norm; None: not).  `grad_norm` holds the norm of the last step (0-d float64) then.
+
+    lr and weight_decay go by parameter group; betas, eps and decoupled_weight_decay are the same for all groups.  State is
+    named and shaped as torch.optim.Adam's (float32 moments for 16-bit parameters), so a state_dict of either loads
+    into the other.  The step counts live on the device: a captured step() counts on with every replay (with the learning
+    rates of its capture)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False,
+                 max_norm=None, norm_type=2.0):
+        if not 0.0 <= lr < math.inf:
+            raise ValueError("FusedAdam: lr must be finite and not negative, got %r" % (lr,))
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("FusedAdam: betas must be in [0, 1), got %r" % (betas,))
+        if not eps >= 0.0:
+            raise ValueError("FusedAdam: eps must not be negative, got %r" % (eps,))
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError("FusedAdam: max_norm must not be negative, got %r" % (max_norm,))
+        self.max_norm, self.norm_type, self.grad_norm = max_norm, norm_type, None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      decoupled_weight_decay=bool(decoupled_weight_decay)))
+
+    def _common(self):
+        first = self.param_groups[0]
+        for g in self.param_groups:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("FusedAdam: amsgrad and maximize are not offered")
+            for k in ("betas", "eps", "decoupled_weight_decay"):
+                if g[k] is not first[k] and g[k] != first[k]:
+                    raise ValueError("FusedAdam: %s has to be the same in all parameter groups" % k)
+        return first
+
+    def _new_state(self, p):
+        s = self.state[p]
+        wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+        s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+        for k in ("exp_avg", "exp_avg_sq"):
+            s[k] = torch.zeros_like(p, dtype=wide, memory_format=torch.preserve_format)
+        return s
+
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        first, state = self._common(), self.state
+        params, grads, avgs, sqs, steps, lr, wd = [], [], [], [], [], [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                s = state.get(p) or self._new_state(p)
+                params.append(p)
+                grads.append(g)
+                avgs.append(s["exp_avg"])
+                sqs.append(s["exp_avg_sq"])
+                steps.append(s["step"])
+                lr.append(group["lr"])
+                wd.append(group["weight_decay"])
+        if params:
+            self.grad_norm = adam_step(params, grads, avgs, sqs, steps, lr, first["betas"], first["eps"], wd,
+                                       first["decoupled_weight_decay"], self.max_norm, self.norm_type)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As Optimizer.load_state_dict, but moments keep their float32 (or float64) values: the base class rounds them to
+        their parameter's type."""
+        super().load_state_dict(state_dict)
+        for g in self.param_groups:
+            g.setdefault("decoupled_weight_decay", self.defaults["decoupled_weight_decay"])
+        self._common()
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            saved = state_dict["state"].get(i)
+            if not saved:
+                continue
+            if "max_exp_avg_sq" in saved:
+                raise ValueError("FusedAdam: amsgrad and maximize are not offered")
+            s = self._new_state(p)
+            s["step"].copy_(torch.as_tensor(saved["step"], dtype=torch.float32))
+            for k in ("exp_avg", "exp_avg_sq"):
+                s[k].copy_(saved[k])

@@ -15,11 +15,13 @@ import torch
 from torch import nn
 from torch.nn.parameter import Parameter
 
+from . import optim
+
 
 def build_optimizer(cfg, named_parameters):
     """solver/build.py:4-25, including its carry-over: `lr` is not reset between parameters, so a parameter
     that follows a "bias" / "sd" one inherits that learning rate (no effect when both factors are 1, as in the
-    reference's yamls)."""
+    reference's yamls).  SOLVER.FUSED: Adam as optim.FusedAdam, which also clips by SOLVER.CLIP_GRAD_NORM."""
     params = []
     lr = cfg.SOLVER.BASE_LR
     for key, value in named_parameters:
@@ -31,7 +33,11 @@ def build_optimizer(cfg, named_parameters):
             lr = cfg.SOLVER.BASE_LR * cfg.SOLVER.STD_LR_FACTOR
         params += [{"params": [value], "lr": lr}]
     if cfg.SOLVER.OPTIMIZER == "sgd":
+        if cfg.SOLVER.FUSED:
+            raise ValueError("SOLVER.FUSED is Adam's (SOLVER.OPTIMIZER 'sgd')")
         return torch.optim.SGD(params, lr)
+    if cfg.SOLVER.FUSED:
+        return optim.FusedAdam(params, lr, betas=tuple(cfg.SOLVER.ADAM_BETAS), max_norm=float(cfg.SOLVER.CLIP_GRAD_NORM) or None)
     return torch.optim.Adam(params, lr, betas=tuple(cfg.SOLVER.ADAM_BETAS))
 
 
@@ -255,17 +261,25 @@ class VariationalOptimization(nn.Module):
         (the multi-GPU trainer passes the flattened all-reduce of parallel.py; the reference is single-process).
         Sharded over G ranks the loss of a shard is weighted local_batch / BATCH_SIZE so that the summed gradient
         is the 1-GPU gradient for the objective loss `R` (batch mean of per-step losses, :204); the REINFORCE
-        baselines of PR / IR / SIR are then per-shard statistics."""
+        baselines of PR / IR / SIR are then per-shard statistics.
+        SOLVER.CLIP_GRAD_NORM > 0 bounds the global norm of the (summed) gradient before the step -- differences through
+        contacts grow with the horizon -- and adds it, as it was before clipping, to the returned statistics."""
         loss, stats = self.loss_functions.get(self.method, self.R_loss)(batch_loss)
         if self.local_batch != self.batch_size:
             loss = loss * (float(self.local_batch) / float(self.batch_size))
         self.optimizer.zero_grad()
         loss.backward()
+        grads = [p.grad for p in self.parameters() if p.grad is not None]
         if grad_sync is not None:
-            grad_sync([p.grad for p in self.parameters() if p.grad is not None])
+            grad_sync(grads)
+        max_norm, norm = float(self.cfg.SOLVER.CLIP_GRAD_NORM), None
+        if max_norm > 0 and not self.cfg.SOLVER.FUSED:
+            norm = optim.clip_grad_norm_(grads, max_norm)
         if self.cfg.SOLVER.OPTIMIZER == "sgd":
             nn.utils.clip_grad_value_(self.parameters(), 1)
         self.optimizer.step()
+        if max_norm > 0:
+            stats["grad_norm"] = float(self.optimizer.grad_norm if norm is None else norm)
         with torch.no_grad():                      # "Make sure sd is not negative" :357-359
             self.sd.data.clamp_(min=self.sd_threshold)
         self.log_prob = torch.zeros(self.local_batch, self.horizon, dtype=torch.float64, device=self.device)

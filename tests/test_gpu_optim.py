@@ -1,0 +1,466 @@
+"""GPU: the optimiser-step operators (optim.py over csrc/optim.hip) against their formulas in 64 bits on the host.
+
+Tolerances.  u = half a step of a type: 2^-53, 2^-24, 2^-8 (bfloat16), 2^-11 (float16), relative.  A sum of n positive
+terms in float64, in any order, is off by at most n 2^-53 relative (each addition rounds once; a square or its conversion adds
+one more); a square root halves it and rounds once: (n + 4) 2^-53 bounds every norm here, the host's own included twice.
+A clipped value is a product rounded once to its type, of a factor that is off by the norm's error and three roundings;
+16-bit values are multiplied in float32 (factor and product: 2 x 2^-24 more).  adam_bounds() counts the update's roundings."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"float64": 2.0 ** -53, "float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+TINY = {"float64": 5e-324, "float32": 2.0 ** -149, "bfloat16": 2.0 ** -133, "float16": 2.0 ** -24}     # a step among subnormals
+TYPES = list(HALF)
+
+
+def _t():
+    import torch
+    import mbrl_amd  # noqa: F401
+    from mbrl_amd import optim
+    return torch, optim
+
+
+def make(sizes, dtypes, seed=0, scale=1.0, misaligned=False, positive=False):
+    """Tensors of these sizes on the GPU, types dealt out in turn; misaligned: slices of one buffer a type, so that they
+    start anywhere."""
+    torch, _ = _t()
+    rng = np.random.default_rng(seed)
+    out, offset = [], {}
+    need = {d: sum(int(np.prod(s)) + 1 for s in sizes) + 7 for d in dtypes}
+    buf = {d: torch.zeros(need[d], dtype=getattr(torch, d), device="cuda") for d in dtypes} if misaligned else {}
+    for i, s in enumerate(sizes):
+        d = dtypes[i % len(dtypes)]
+        x = rng.standard_normal(s) * scale * 10.0 ** rng.uniform(-2, 1)
+        x = torch.from_numpy(np.asarray(np.abs(x) if positive else x)).to(getattr(torch, d)).cuda()
+        if misaligned:
+            o = offset.get(d, 1)
+            view = buf[d][o:o + x.numel()].view(x.shape)
+            view.copy_(x)
+            offset[d] = o + x.numel() + i % 2
+            x = view
+        out.append(x)
+    return out
+
+
+def host(ts):
+    return [t.detach().double().cpu().numpy().astype(np.float64) for t in ts]
+
+
+def ref_norm(arrays, p):
+    flat = np.concatenate([a.reshape(-1) for a in arrays] + [np.zeros(0)]).astype(np.longdouble)
+    if not flat.size:
+        return 0.0
+    if p == math.inf:
+        return float(np.max(np.abs(flat)))
+    return float(np.sum(np.abs(flat) ** int(p)) ** (np.longdouble(1) / int(p)))
+
+
+def norm_tol(arrays):
+    return (sum(a.size for a in arrays) + 4) * 2.0 ** -53
+
+
+ODD = [(0,), (1,), (3,), (7, 5), (64,), (257,), (511,), (512,), (513,), (3, 0, 2), (1025,), (63, 65)]
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("dtypes", [[t] for t in TYPES] + [TYPES])
+@pytest.mark.parametrize("misaligned", [False, True])
+def test_norm(p, dtypes, misaligned):
+    _, optim = _t()
+    ts = make(ODD, dtypes, misaligned=misaligned)
+    arrays = host(ts)
+    got = optim.grad_norm(ts, p)
+    assert got.shape == () and str(got.dtype) == "torch.float64"
+    want = ref_norm(arrays, p)
+    assert abs(float(got) - want) <= (0.0 if p == math.inf else norm_tol(arrays) * want)
+
+
+@pytest.mark.parametrize("n", [1, 4095, 4096, 4097, 70001, 300007])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_and_clip_of_one_tensor(n, dtype):
+    check_clip([(n,)], [dtype], 0.3)
+
+
+def check_clip(sizes, dtypes, fraction, p=2.0, misaligned=False, seed=1):
+    _, optim = _t()
+    ts = make(sizes, dtypes, seed=seed, misaligned=misaligned)
+    arrays = host(ts)
+    want = ref_norm(arrays, p)
+    most = fraction * want
+    norm = optim.clip_grad_norm_(ts, most, p)
+    assert abs(float(norm) - want) <= norm_tol(arrays) * want
+    c = min(1.0, most / (want + 1e-6))
+    for t, a in zip(ts, arrays):
+        name = str(t.dtype)[6:]
+        rel = HALF[name] + norm_tol(arrays) + 4 * 2.0 ** -53 + (2 * 2.0 ** -24 if name in ("bfloat16", "float16") else 0.0)
+        got = t.double().cpu().numpy()
+        if fraction > 1.0:
+            assert np.array_equal(got, a)
+        else:
+            assert np.all(np.abs(got - a * c) <= 1.001 * rel * np.abs(a * c) + TINY[name]), name
+    return ts
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("dtypes", [[t] for t in TYPES] + [TYPES])
+@pytest.mark.parametrize("fraction", [0.3, 0.0, 3.0])
+def test_clip(p, dtypes, fraction):
+    check_clip(ODD, dtypes, fraction, p)
+    check_clip(ODD, dtypes, fraction, p, misaligned=True)
+
+
+@pytest.mark.parametrize("count", [64, 65, 191, 192, 193, 400, 1000])
+def test_many_tensors(count):
+    """Around the borders of what one launch takes, and of one wave's search for a unit's tensor."""
+    rng = np.random.default_rng(count)
+    sizes = [(int(rng.integers(0, 700)),) for _ in range(count)]
+    check_clip(sizes, TYPES, 0.4, misaligned=True)
+    check_adam(sizes, ["float32", "bfloat16"], most=0.5, misaligned=True)
+
+
+def test_empty_lists_and_zeros():
+    torch, optim = _t()
+    for ts in ([], [torch.zeros(0, device="cuda")], [torch.zeros((0, 4), device="cuda", dtype=torch.float16)] * 3):
+        assert float(optim.grad_norm(ts)) == 0.0 and float(optim.clip_grad_norm_(ts, 1.0)) == 0.0
+    ts = [torch.zeros(100, device="cuda"), -torch.zeros(3, device="cuda", dtype=torch.float64)]
+    for p in (1, 2, math.inf):
+        assert float(optim.grad_norm(ts, p)) == 0.0
+    assert float(optim.clip_grad_norm_(ts, 1.0)) == 0.0 and all(not bool(t.any()) for t in ts)
+    assert optim.adam_step([], [], [], [], [], 1e-3) is None
+    assert float(optim.adam_step([], [], [], [], [], 1e-3, max_norm=1.0)) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+def test_nan_and_infinity(dtype, p):
+    torch, optim = _t()
+    for bad, n in ((math.nan, 5), (math.inf, 5000), (-math.inf, 700)):
+        ts = make([(33,), (n,)], [dtype], seed=3)
+        ts[1][n - 1] = bad
+        norm = float(optim.grad_norm(ts, p))
+        assert math.isnan(norm) if math.isnan(bad) else norm == math.inf
+        with pytest.raises(RuntimeError, match="norm of the gradients"):
+            optim.clip_grad_norm_(ts, 1.0, p, error_if_nonfinite=True)
+        keep = host(ts)
+        optim.clip_grad_norm_(ts, 1.0, p)
+        got = host(ts)
+        if math.isnan(bad):
+            assert all(np.isnan(a).all() for a in got)
+        else:
+            assert not got[0].any() and not got[1][:-1].any() and np.isnan(got[1][-1]) and np.isfinite(keep[0]).all()
+    # both: a NaN wins over an infinity wherever they are
+    ts = make([(3,), (900,)], [dtype], seed=4)
+    ts[0][1], ts[1][890] = math.inf, math.nan
+    assert math.isnan(float(optim.grad_norm(ts, p)))
+    ts[0][1], ts[1][890] = math.nan, math.inf
+    assert math.isnan(float(optim.grad_norm(ts, p)))
+
+
+def test_largest_and_smallest_values():
+    torch, optim = _t()
+    x = torch.full((1000,), 3e38, device="cuda")
+    assert float(optim.grad_norm([x])) == pytest.approx(float(np.float32(3e38)) * math.sqrt(1000), rel=1e-12)
+    assert float(optim.grad_norm([x.bfloat16()])) == pytest.approx(float(x.bfloat16()[0]) * math.sqrt(1000), rel=1e-12)
+    optim.clip_grad_norm_([x], 1.0)
+    assert np.allclose(x.cpu().numpy(), 1 / math.sqrt(1000), rtol=2.0 ** -23, atol=0)
+    s = torch.full((77,), 1e-45, device="cuda")                     # a subnormal: not flushed
+    assert float(optim.grad_norm([s])) == pytest.approx(float(s[0]) * math.sqrt(77), rel=1e-12) and float(s[0]) > 0
+    d = torch.tensor([1e300, 1.0], dtype=torch.float64, device="cuda")
+    assert float(optim.grad_norm([d])) == math.inf and float(optim.grad_norm([d], math.inf)) == 1e300
+
+
+def test_any_dense_order_of_values():
+    torch, optim = _t()
+    base = make([(6, 10, 4)], ["float32"], seed=8)[0]
+    for x in (base.permute(2, 0, 1).contiguous().permute(1, 2, 0), base.clone().t() if base.dim() == 2 else base.clone().transpose(0, 2)):
+        a = x.cpu().numpy().astype(np.float64)
+        norm = optim.clip_grad_norm_([x], 0.5 * ref_norm([a], 2))
+        c = 0.5 * ref_norm([a], 2) / (float(norm) + 1e-6)
+        assert np.all(np.abs(x.double().cpu().numpy() - c * a) <= 1.01 * 2.0 ** -24 * np.abs(c * a))
+    rows = base.view(6, 40)[2]                                       # a row of a matrix: the rest stays as it was
+    keep = base.clone()
+    optim.clip_grad_norm_([rows], 0.0)
+    assert not bool(base.view(6, 40)[2].any()) and torch.equal(base.view(6, 40)[3:], keep.view(6, 40)[3:])
+    assert torch.equal(base.view(6, 40)[:2], keep.view(6, 40)[:2])
+
+
+def test_same_bits_every_time_and_shared_memory_is_refused():
+    torch, optim = _t()
+    ts = make([(100003,), (999,), (40, 6)], TYPES, seed=5)
+    norms = {float(optim.grad_norm(ts, p)) for _ in range(20) for p in (2,)}
+    assert len(norms) == 1
+    x = torch.ones(100, device="cuda")
+    # counted twice where it is only read: sqrt(200) from two exact sums of 100, one rounding
+    assert float(optim.grad_norm([x, x])) == math.sqrt(200.0)
+    for pair in ([x, x], [x[:60], x[50:]], [x, x[3:4]]):
+        with pytest.raises(ValueError, match="share memory"):
+            optim.clip_grad_norm_(pair, 1.0)
+    assert bool((x == 1).all())
+    optim.clip_grad_norm_([x[:50], x[50:]], 1.0)
+    step = torch.zeros((), device="cuda")
+    y = [torch.ones(100, device="cuda") for _ in range(6)]
+    with pytest.raises(ValueError, match="shares memory"):
+        optim.adam_step(y[:2], y[2:4], y[4:5] * 2, [y[5], torch.ones(100, device="cuda")], [step, step.clone()], 1e-3)
+    with pytest.raises(ValueError, match="shares memory"):       # one counter for two parameters
+        optim.adam_step(y[:2], y[2:4], y[4:], [torch.ones(100, device="cuda") for _ in range(2)], [step, step], 1e-3)
+
+
+# ---- Adam ----
+def adam_bounds(x, g, m, v, t, lr, b1, b2, eps, wd, decoupled, c, u, c_err):
+    """One step in extended precision (so that float64 results can be held to their own roundings) and the largest errors, with
+    u the half step of the arithmetic.
+    g1 = c g: factor rounded, product: 2u (and the factor's own error).  L2: wd rounded, one fused product: 2u |wd x| + u |g1|.
+    m': a1 = 1 - b1 rounded, a1 g1 rounded, b1 rounded, one fused sum.
+    v': a2 rounded, two products, g1 squared (twice its error); b2 rounded; one fused sum.
+    d = sqrt(v') root + eps: half of v's error, sqrt, root and eps rounded, one fused sum.
+    x' = x keep - size (m' / d): quotient, size, keep, product, one fused sum.
+    size and root come from 1 - b^t = -expm1(t log1p(b - 1)) in float64: log1p and expm1 within a step (2 w with w = 2^-53), the
+    product w, and expm1 of a negative number passes on at most its argument's relative error: 5 w, a division (and a root)
+    more: 6 w.  keep = 1 - lr wd: two roundings."""
+    x, g, m, v = (a.astype(np.longdouble) for a in (x, g, m, v))
+    b1, b2, one, w = np.longdouble(b1), np.longdouble(b2), np.longdouble(1), 2.0 ** -53
+    g1 = np.longdouble(c) * g
+    eg = (2 * u + c_err) * np.abs(g1)
+    if not decoupled and wd:
+        g1 = g1 + np.longdouble(wd) * x
+        eg = eg + 2 * u * np.abs(wd * x) + u * np.abs(g1)
+    m1 = b1 * m + (1 - b1) * g1
+    em = 2 * u * np.abs(b1 * m) + (1 - b1) * (eg + 2 * u * np.abs(g1)) + u * np.abs(m1)
+    v1 = b2 * v + (1 - b2) * g1 * g1
+    ev = 2 * u * b2 * v + (1 - b2) * (2 * np.abs(g1) * eg + eg * eg + 4 * u * g1 * g1) + u * v1
+    root = one / np.sqrt(one - b2 ** t)
+    s = np.sqrt(v1)
+    es = np.where(v1 > 0, ev / (2 * np.where(v1 > 0, s, 1)), np.sqrt(ev)) + u * s
+    d = s * root + eps
+    ed = es * root + (3 * u + 6 * w) * s * root + u * eps + u * d
+    size = lr / (one - b1 ** t)
+    q = m1 / d
+    eq = em / d + np.abs(q) * ed / d + u * np.abs(q)
+    keep = one - np.longdouble(lr) * np.longdouble(wd) if decoupled else one
+    x1 = x * keep - size * q
+    ex = size * eq + (2 * u + 6 * w) * size * np.abs(q) + 3 * u * np.abs(x * keep) * (1 if decoupled else 0) + u * np.abs(x1)
+    return (x1, 1.02 * ex), (m1, 1.02 * em), (v1, 1.02 * ev)
+
+
+def check_adam(sizes, dtypes, most=None, p=2.0, wd=0.0, decoupled=False, misaligned=False, steps=2, seed=11, lrs=(1e-3, 1e-2)):
+    torch, optim = _t()
+    wide = lambda d: "float64" if d == "float64" else "float32"      # noqa: E731
+    xs = make(sizes, dtypes, seed, misaligned=misaligned)
+    ms = [t.to(getattr(torch, wide(str(x.dtype)[6:]))).mul_(0.1) for t, x in zip(make(sizes, dtypes, seed + 1), xs)]
+    vs = [t.to(getattr(torch, wide(str(x.dtype)[6:]))).square_().mul_(0.1) for t, x in zip(make(sizes, dtypes, seed + 2), xs)]
+    counts = [torch.tensor(float(i % 5), device="cuda") for i in range(len(sizes))]
+    lr = [lrs[i % len(lrs)] for i in range(len(sizes))]
+    b1, b2, eps = 0.9, 0.99, 1e-6
+    for k in range(steps):
+        gs = make(sizes, dtypes, seed + 10 + k, misaligned=misaligned)
+        ax, ag, am, av = host(xs), host(gs), host(ms), host(vs)
+        limit = None if most is None else most * ref_norm(ag, p)
+        versions = [x._version for x in xs]
+        norm = optim.adam_step(xs, gs, ms, vs, counts, lr, (b1, b2), eps, wd, decoupled, limit, p)
+        c, c_err = 1.0, 0.0
+        if most is None:
+            assert norm is None
+        else:
+            want = ref_norm(ag, p)
+            assert abs(float(norm) - want) <= norm_tol(ag) * want
+            c, c_err = min(1.0, limit / (want + 1e-6)), norm_tol(ag) + 4 * 2.0 ** -53
+        for i, (x, g, m, v) in enumerate(zip(xs, gs, ms, vs)):
+            name, t = str(x.dtype)[6:], i % 5 + k + 1
+            assert float(counts[i]) == t and x._version > versions[i]     # views of one buffer count together
+            assert np.array_equal(g.double().cpu().numpy(), ag[i])                    # gradients are only read
+            bounds = adam_bounds(ax[i], ag[i], am[i], av[i], t, lr[i], b1, b2, eps, wd, decoupled, c, HALF[wide(name)], c_err)
+            for what, got, (ref, err), extra in (("x", x, bounds[0], HALF[name] if name != wide(name) else 0.0), ("m", m, bounds[1], 0.0),
+                                                 ("v", v, bounds[2], 0.0)):
+                got = got.double().cpu().numpy().astype(np.longdouble)
+                slack = err + extra * (np.abs(ref) + err) + TINY[name if what == "x" else wide(name)]
+                assert np.all(np.abs(got - ref) <= slack), (what, name, sizes[i], float(np.max(np.abs(got - ref) / slack)))
+
+
+@pytest.mark.parametrize("dtypes", [[t] for t in TYPES] + [TYPES])
+@pytest.mark.parametrize("wd,decoupled", [(0.0, False), (0.1, False), (0.1, True)])
+@pytest.mark.parametrize("most", [None, 0.3, 3.0])
+def test_adam(dtypes, wd, decoupled, most):
+    check_adam(ODD, dtypes, most, wd=wd, decoupled=decoupled)
+
+
+@pytest.mark.parametrize("p", [1.0, math.inf])
+def test_adam_clips_by_other_norms(p):
+    check_adam(ODD, TYPES, 0.3, p, misaligned=True)
+
+
+@pytest.mark.parametrize("count", [79, 80, 81, 159, 160, 161])
+def test_adam_list_borders(count):
+    check_adam([(1 + 37 * i % 90,) for i in range(count)], TYPES, misaligned=True)
+
+
+@pytest.mark.parametrize("n", [4095, 8193, 70001, 1 << 20])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_adam_of_one_tensor(n, dtype):
+    check_adam([(n,)], [dtype], 0.5)
+
+
+def test_adam_keeps_infinite_parameters_apart_from_their_moments():
+    torch, optim = _t()
+    x, g = torch.full((5,), math.inf, device="cuda"), torch.ones(5, device="cuda")
+    m, v, t = torch.zeros(5, device="cuda"), torch.zeros(5, device="cuda"), torch.zeros((), device="cuda")
+    optim.adam_step([x], [g], [m], [v], [t], 1e-3)
+    assert bool(torch.isinf(x).all()) and np.allclose(m.cpu(), 0.1) and np.allclose(v.cpu(), 1e-3)
+    # a first step of size lr whatever the gradient's scale; nothing where there has never been a gradient
+    x, g = torch.zeros(4, device="cuda"), torch.tensor([1e-3, -1e3, 0.0, 1.0], device="cuda")
+    m, v, t = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros((), device="cuda")
+    optim.adam_step([x], [g], [m], [v], [t], 0.5)
+    assert np.allclose(x.cpu(), [-0.5, 0.5, 0.0, -0.5], rtol=2e-5)
+
+
+def test_fused_adam_follows_torchs_adam():
+    """Same rule, other rounding: float64 parameters agree to 1e-12 relative over 25 steps (about 30 roundings of 2^-53 a
+    step on values of order 1, no cancellation beyond the update's own size); parameters without a gradient rest."""
+    torch, optim = _t()
+    for wd, decoupled in ((0.0, False), (0.02, False), (0.02, True)):
+        a = [t.clone().requires_grad_() for t in make([(6, 40), (6, 40), (17,), (4, 3, 2)], ["float64"], 21)]
+        b = [t.detach().clone().requires_grad_() for t in a]
+        kw = dict(betas=(0.85, 0.97), eps=1e-7, weight_decay=wd, decoupled_weight_decay=decoupled)
+        mine = optim.FusedAdam([{"params": a[:2], "lr": 0.01}, {"params": a[2:], "lr": 0.003}], **kw)
+        ref = torch.optim.Adam([{"params": b[:2], "lr": 0.01}, {"params": b[2:], "lr": 0.003}], **kw)
+        for k in range(25):
+            gs = make([tuple(t.shape) for t in a], ["float64"], 100 + k)
+            for i, (x, y, g) in enumerate(zip(a, b, gs)):
+                x.grad, y.grad = (None, None) if i == 2 and k % 3 else (g, g.clone())
+            mine.step()
+            ref.step()
+            if k == 12:                       # each goes on from the other's state
+                s, r = mine.state_dict(), ref.state_dict()
+                mine.load_state_dict(r)
+                ref.load_state_dict(s)
+        for x, y in zip(a, b):
+            assert torch.allclose(x, y, rtol=1e-12, atol=1e-12)
+            assert float(mine.state[x]["step"]) == float(ref.state[y]["step"])
+
+
+def test_captured_and_replayed():
+    """Both calls in one graph, replayed with eager work and a second graph between the replays: the counters go on, and each
+    replay gives the bits of the eager calls."""
+    torch, optim = _t()
+    sizes = [(300, 7), (513,), (100001,), (0,)]
+
+    def state():
+        xs, gs = make(sizes, ["float32", "float64"], 31), make(sizes, ["float32", "float64"], 32)
+        return xs, gs, [torch.zeros_like(x) for x in xs], [torch.zeros_like(x) for x in xs], [torch.zeros((), device="cuda") for _ in xs]
+
+    def one(s):
+        n = optim.clip_grad_norm_(s[1], 5.0)
+        return n, optim.adam_step(*s, 0.01, max_norm=2.0, norm_type=1)
+    eager, graphs, norms = state(), [], []
+    states = [state(), state()]
+    for s in states:
+        warm = [[t.clone() for t in l] for l in s]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one(warm)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            norms.append(one(s))
+        graphs.append(g)
+    for k in range(5):
+        fresh = make(sizes, ["float32", "float64"], 50 + k)
+        for l in (eager, *states):
+            for a, b in zip(l[1], fresh):
+                a.copy_(b)
+        want = one(eager)
+        for g in graphs:
+            g.replay()
+        one([[t.clone() for t in l] for l in eager])           # eager work of the same kind between
+        torch.cuda.synchronize()
+        for s, n in zip(states, norms):
+            assert float(n[0]) == float(want[0]) and float(n[1]) == float(want[1])
+            for la, lb in zip(s, eager):
+                for a, b in zip(la, lb):
+                    assert torch.equal(a, b), k
+        assert float(eager[4][0]) == k + 1
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(ValueError, match="captured"):
+            optim.clip_grad_norm_(eager[1], 1.0, error_if_nonfinite=True)
+
+
+def test_streams_beside_each_other():
+    torch, optim = _t()
+    lists = [make([(200003,), (77,)], ["float32"], 60 + i) for i in range(4)]
+    want = [host(l) for l in lists]
+    streams = [torch.cuda.Stream() for _ in lists]
+    torch.cuda.synchronize()
+    norms = []
+    for l, s in zip(lists, streams):
+        with torch.cuda.stream(s):
+            norms.append([optim.clip_grad_norm_(l, 1.0) for _ in range(3)])
+    torch.cuda.synchronize()
+    for l, a, n in zip(lists, want, norms):
+        assert abs(float(n[0]) - ref_norm(a, 2)) <= norm_tol(a) * ref_norm(a, 2)
+        # clipped once: under the bound from then on, but for the rounding of 2e5 values
+        assert abs(float(n[1]) - 1.0) < 2e-6 and float(n[2]) <= 1.0 + 2.0 ** -24
+
+
+def test_more_values_than_32_bits_count():
+    """One float16 tensor of 2^31 + 4099 values (4 GiB): the last ones count, and are reached."""
+    torch, optim = _t()
+    n = (1 << 31) + 4099
+    x = torch.zeros(n, dtype=torch.float16, device="cuda")
+    at = [0, (1 << 31) - 1, 1 << 31, (1 << 31) + 4096, n - 1]
+    x[at] = 3.0
+    assert float(optim.grad_norm([x])) == math.sqrt(45.0)
+    optim.clip_grad_norm_([x], 0.5 * (math.sqrt(45.0) + 1e-6))
+    assert x[at].tolist() == [1.5] * 5 and int(torch.count_nonzero(x)) == 5
+
+
+def test_a_run_of_them_together():
+    """What a training loop does with them: gradients by autograd, their norm, clipping, update -- against the same in float64
+    on the host, which starts every step from the same weights."""
+    torch, optim = _t()
+    torch.manual_seed(0)
+    from mbrl_amd.strategies import FeedForward
+    net = FeedForward(18, [64, 64, 32, 8], 6).cuda()
+    ref = FeedForward(18, [64, 64, 32, 8], 6).double()
+    ref.load_state_dict({k: v.double().cpu() for k, v in net.state_dict().items()})
+    opt, oref = optim.FusedAdam(net.parameters(), 1e-3, max_norm=0.25), torch.optim.Adam(ref.parameters(), 1e-3, foreach=False)
+    data = torch.randn(5, 64, 18)
+    for k in range(5):
+        ref.load_state_dict({k: v.double().cpu() for k, v in net.state_dict().items()})
+        for model, o, x in ((net, opt, data[k].cuda()), (ref, oref, data[k].double())):
+            o.zero_grad()
+            (model(x) ** 2).sum().backward()
+        before = optim.grad_norm([p.grad for p in net.parameters()])
+        opt.step()
+        want = torch.nn.utils.clip_grad_norm_(ref.parameters(), 0.25)
+        oref.step()
+        assert float(opt.grad_norm) == float(before)
+        assert float(before) == pytest.approx(float(want), rel=1e-3)        # float32 network against float64
+        first = optim.clip_grad_norm_([p.grad for p in net.parameters()], 0.25)
+        assert float(first) == float(before)
+        assert float(optim.grad_norm([p.grad for p in net.parameters()])) <= 0.25 * (1 + 2.0 ** -22)
+        # an entry of Adam's step is at most lr (1 - b1) / sqrt(1 - b2) = 3.2 lr: where a gradient's sign is rounding, the two differ by twice that
+        off = torch.cat([(p.detach().double().cpu() - q.detach()).abs().reshape(-1) for p, q in zip(net.parameters(), ref.parameters())])
+        assert float(off.max()) <= 2 * 3.2e-3 and float(off.median()) <= 1e-5
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_trainer_clips(fused, tmp_path):
+    """do_training with SOLVER.CLIP_GRAD_NORM: the same parameters whether torch's Adam follows the clipping or the fused
+    update clips on its way, and every step's norm within the bound changes nothing against no clipping at all."""
+    torch, optim = _t()
+    from test_gpu_trainer import _cfg, _train
+    base = dict(SOLVER__BASE_LR=0.02, MODEL__POLICY__NETWORK=False)
+    res = {}
+    for tag, over in (("torch", dict(SOLVER__CLIP_GRAD_NORM=1e-3)), ("fused", dict(SOLVER__CLIP_GRAD_NORM=1e-3, SOLVER__FUSED=True)),
+                      ("idle", dict(SOLVER__CLIP_GRAD_NORM=1e12, SOLVER__FUSED=fused)), ("none", dict(SOLVER__FUSED=fused))):
+        agent, rows, d = _train(_cfg("InvertedDoublePendulumEnv", **base, **over), tmp_path, tag)
+        res[tag] = {k: v.cpu().double() for k, v in agent.policy_net.state_dict().items()}
+        assert type(agent.policy_net.optimizer) is (optim.FusedAdam if over.get("SOLVER__FUSED") else torch.optim.Adam)
+    for k in res["torch"]:
+        assert torch.allclose(res["torch"][k], res["fused"][k], rtol=1e-6, atol=1e-9), k
+        assert torch.equal(res["idle"][k], res["none"][k]), k
+        assert torch.isfinite(res["fused"][k]).all()
