@@ -31,7 +31,12 @@ using mbrl::report;
 
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMaxBlocks = 1024;          // of a launch: 4 blocks of 4 waves a CU
-constexpr int kMinShift = 9, kMaxShift = 12;
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
+constexpr int kMinShift = 9, kMaxShift = 12, kSmallShift = 8;
+constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;      // bytes that one block takes on alone
+constexpr int kMaxParts = 2048;           // partial sums that every block of a second launch joins for itself
+constexpr int64_t kCache = int64_t(256) << 20;                   // bytes of the last-level cache
+constexpr int kStreamBlocks = 1 << 22;    // of a launch that does not stay: HIP counts threads in 32 bits
 
 // ---- element types: what is stored, what is computed with, values in 16 bytes ----
 struct F64 { using T = double; using C = double; static constexpr int V = 2; };
@@ -42,14 +47,20 @@ struct F16 { using T = _Float16; using C = float; static constexpr int V = 8; };
 // Vectors with the alignment of their elements: a tensor may start at any element (a slice of a bucket), and the memory
 // system takes a 16-byte access at any such address, so there is one path for all alignments.
 template <class T, int V> struct Pack { T v[V]; };
-template <class T, int V>
+template <int kBytes, int kAlign> struct Raw { typedef uint32_t type __attribute__((ext_vector_type(kBytes / 4), aligned(kAlign))); };
+template <bool kStream, int V, class T>
 __device__ __forceinline__ Pack<T, V> load(const T *p) {
-    Pack<T, V> r;
-    __builtin_memcpy(&r, p, sizeof r);
-    return r;
+    using R = typename Raw<int(sizeof(Pack<T, V>)), int(sizeof(T))>::type;
+    const R *q = reinterpret_cast<const R *>(p);
+    return __builtin_bit_cast(Pack<T, V>, kStream ? __builtin_nontemporal_load(q) : *q);
 }
-template <class T, int V>
-__device__ __forceinline__ void store(T *p, const Pack<T, V> &r) { __builtin_memcpy(p, &r, sizeof r); }
+template <bool kStream, int V, class T>
+__device__ __forceinline__ void store(T *p, const Pack<T, V> &r) {
+    using R = typename Raw<int(sizeof(Pack<T, V>)), int(sizeof(T))>::type;
+    R *q = reinterpret_cast<R *>(p);
+    if (kStream) __builtin_nontemporal_store(__builtin_bit_cast(R, r), q);
+    else *q = __builtin_bit_cast(R, r);
+}
 
 // Calls f(integral_constant-like element type) for a stored type code; wave-uniform.
 template <class F>
@@ -61,26 +72,29 @@ __device__ __forceinline__ void by_type(int code, F &&f) {
 }
 
 // ---- lists in kernel arguments ----
-template <int K> struct Units {
+template <int K_> struct Units {
+    static constexpr int K = K_;
     uint64_t n[K];        // values << 2 | type code
     uint32_t end[K];      // units of the tensors up to and including this one
     int count, shift;
     uint32_t units;
 };
-constexpr int kNormList = 192, kAdamList = 80, kStepList = 160;
-struct NormList { Units<kNormList> u; void *x[kNormList]; };
-struct AdamList { Units<kAdamList> u; void *p[kAdamList]; const void *g[kAdamList]; void *m[kAdamList], *v[kAdamList]; uint32_t s[kAdamList]; };
-struct StepList { float *step[kStepList]; double lr[kStepList], wd[kStepList]; int count; };
-static_assert(sizeof(NormList) <= 3968 && sizeof(AdamList) <= 3968 && sizeof(StepList) <= 3968, "kernel arguments are 4 KB");
+template <int K> struct NormList { Units<K> u; void *x[K]; };
+template <int K> struct BeginList { Units<K> u; const void *x[K]; float *step[K]; double lr[K], wd[K]; };       // x: gradients
+template <int K> struct UpdateList { Units<K> u; const void *x[K]; void *p[K], *m[K], *v[K]; };
+template <int K> struct StepList { UpdateList<K> l; float *step[K]; double lr[K], wd[K]; };                     // both, for one launch
+constexpr int kFew = 16, kNormList = 192, kAdamList = 80, kStepList = 52;
+static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kAdamList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
+              sizeof(StepList<kStepList>) <= 3968, "kernel arguments are 4 KB");
 
-// What the update of one tensor multiplies with (adam_scalars).
+// What the update of one tensor multiplies with.
 struct Scalars { double size, root, keep, l2; };
 
 __device__ __forceinline__ uint32_t wave_of_block() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
 
 // The tensor that unit `unit` belongs to: as many as end at or before it come first.
-template <int K>
-__device__ __forceinline__ int owner(const Units<K> &u, uint32_t unit) {
+template <class U>
+__device__ __forceinline__ int owner(const U &u, uint32_t unit) {
     const int lane = threadIdx.x % kWave;
     int t = 0;
     for (int k = 0; k < u.count; k += kWave)
@@ -88,18 +102,36 @@ __device__ __forceinline__ int owner(const Units<K> &u, uint32_t unit) {
     return __builtin_amdgcn_readfirstlane(t);
 }
 
-// One unit of a list: its tensor, its first value and how many it has.
+// Values of one tensor, one after another.
 struct Piece { int t, type; int64_t first; int n; };
-template <int K>
-__device__ __forceinline__ Piece piece(const Units<K> &u, uint32_t unit) {
+
+// Units `unit` to `stop` of the list, as far as they lie in one tensor; moves `unit` past them.
+template <class U>
+__device__ __forceinline__ Piece piece(const U &u, uint32_t &unit, uint32_t stop) {
     Piece p;
     p.t = owner(u, unit);
     const uint64_t n = u.n[p.t];
+    const uint32_t end = min(stop, u.end[p.t]), skipped = unit - (p.t ? u.end[p.t - 1] : 0);
     p.type = int(n & 3);
-    p.first = int64_t(unit - (p.t ? u.end[p.t - 1] : 0)) << u.shift;
-    const int64_t left = int64_t(n >> 2) - p.first;
-    p.n = int(left < (int64_t(1) << u.shift) ? left : (int64_t(1) << u.shift));
+    p.first = int64_t(skipped) << u.shift;
+    p.n = int(min(int64_t(n >> 2) - p.first, int64_t(end - unit) << u.shift));
+    unit = end;
     return p;
+}
+
+// The share of wave `wave` of `waves`: every waves-th unit, so that waves that run together read what lies together.
+template <class U, class F>
+__device__ __forceinline__ void dealt(const U &u, uint32_t wave, uint32_t waves, F f) {
+    for (uint32_t i = wave; i < u.units; i += waves) {
+        uint32_t unit = i;
+        f(piece(u, unit, unit + 1));
+    }
+}
+// The same for the waves of one block: units one after another, so that each has few tensors to find.
+template <class U, class F>
+__device__ __forceinline__ void shared_out(const U &u, uint32_t wave, F f) {
+    const uint32_t each = (u.units + kSmallWaves - 1) / kSmallWaves, stop = min(u.units, (wave + 1) * each);
+    for (uint32_t unit = wave * each; unit < stop;) f(piece(u, unit, stop));
 }
 
 // ---- norm ----
@@ -120,37 +152,38 @@ __device__ __forceinline__ double add(double acc, double x) {
     return larger(acc, fabs(x));
 }
 
-template <int P>
+// Every thread gets the join of all threads' values; W: waves of the block.
+template <int P, int W>
 __device__ __forceinline__ double block_join(double a) {
-    __shared__ double part[kWaves];
+    __shared__ double part[W];
     for (int d = kWave / 2; d; d /= 2) a = join<P>(a, __shfl_xor(a, d));
     __syncthreads();
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = a;
     __syncthreads();
     a = part[0];
-    for (int w = 1; w < kWaves; w++) a = join<P>(a, part[w]);
+    for (int w = 1; w < W; w++) a = join<P>(a, part[w]);
     return a;
 }
 
-template <int P, class E>
-__device__ __forceinline__ double unit_norm(E, const void *base, int64_t first, int n, double acc) {
+template <int P, bool kStream, class E>
+__device__ __forceinline__ double piece_norm(E, const void *base, const Piece &p, double acc) {
     using T = typename E::T;
     constexpr int V = E::V, kStep = kWave * V;
-    const T *x = static_cast<const T *>(base) + first;
-    const int lane = threadIdx.x % kWave;
+    const T *x = static_cast<const T *>(base) + p.first;
+    const int lane = threadIdx.x % kWave, n = p.n;
     int i = lane * V;
     double a[2] = {acc, 0.0};
     for (; i + 3 * kStep + V <= n; i += 4 * kStep) {
         Pack<T, V> r[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) r[k] = load<T, V>(x + i + k * kStep);
+        for (int k = 0; k < 4; k++) r[k] = load<kStream, V>(x + i + k * kStep);
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
             for (int j = 0; j < V; j++) a[j % 2] = add<P>(a[j % 2], double(typename E::C(r[k].v[j])));
     }
     for (; i + V <= n; i += kStep) {
-        const Pack<T, V> r = load<T, V>(x + i);
+        const Pack<T, V> r = load<kStream, V>(x + i);
 #pragma unroll
         for (int j = 0; j < V; j++) a[j % 2] = add<P>(a[j % 2], double(typename E::C(r.v[j])));
     }
@@ -159,102 +192,149 @@ __device__ __forceinline__ double unit_norm(E, const void *base, int64_t first, 
     return join<P>(a[0], a[1]);
 }
 
-template <int P>
-__global__ __launch_bounds__(kThreads) void norm_partials(const NormList l, double *part) {
+__device__ __forceinline__ uint32_t wave_of_grid() { return blockIdx.x * kWaves + wave_of_block(); }
+__device__ __forceinline__ uint32_t waves_of_grid() { return gridDim.x * kWaves; }
+
+template <int P, bool kStream, class L>
+__device__ __forceinline__ double grid_norm(const L &l) {
     double acc = 0.0;
-    for (uint32_t unit = blockIdx.x * kWaves + wave_of_block(); unit < l.u.units; unit += gridDim.x * kWaves) {
-        const Piece p = piece(l.u, unit);
-        by_type(p.type, [&](auto e) { acc = unit_norm<P>(e, l.x[p.t], p.first, p.n, acc); });
-    }
-    acc = block_join<P>(acc);
+    dealt(l.u, wave_of_grid(), waves_of_grid(), [&](const Piece &p) {
+        by_type(p.type, [&](auto e) { acc = piece_norm<P, kStream>(e, l.x[p.t], p, acc); });
+    });
+    return block_join<P, kWaves>(acc);
+}
+template <int P, class L>
+__device__ __forceinline__ double small_norm(const L &l) {
+    double acc = 0.0;
+    shared_out(l.u, wave_of_block(), [&](const Piece &p) {
+        by_type(p.type, [&](auto e) { acc = piece_norm<P, false>(e, l.x[p.t], p, acc); });
+    });
+    return block_join<P, kSmallWaves>(acc);
+}
+
+template <int P, bool kStream, class L>
+__global__ __launch_bounds__(kThreads) void norm_partials(const L l, double *part) {
+    const double acc = grid_norm<P, kStream>(l);
     if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
-// The partial sums in their order -> the norm, and the factor that clipping multiplies with.  A norm that is not a number
-// makes the factor NaN (the comparison is false), an infinite one makes it 0.
+template <int P> __device__ __forceinline__ double root_of(double acc) { return P == MBRL_NORM_TWO ? sqrt(acc) : acc; }
+
+// What clipping multiplies with.  A norm that is not a number makes it NaN (the comparison is false), an infinite one 0.
+__device__ __forceinline__ double factor_of(double norm, double max_norm) {
+    const double c = max_norm / (norm + 1e-6);
+    return c > 1.0 ? 1.0 : c;
+}
+
+// The partial sums in their order.
 template <int P>
-__global__ __launch_bounds__(kThreads) void norm_finish(const double *part, int count, double max_norm, double *norm, double *factor) {
+__device__ __forceinline__ double join_partials(const double *part, int parts) {
+    if (parts == 1) return part[0];
     double acc = 0.0;
-    for (int i = threadIdx.x; i < count; i += kThreads) acc = join<P>(acc, part[i]);
-    acc = block_join<P>(acc);
+    for (int i = threadIdx.x; i < parts; i += kThreads) acc = join<P>(acc, part[i]);
+    return block_join<P, kWaves>(acc);
+}
+
+template <int P>
+__global__ __launch_bounds__(kThreads) void norm_finish(const double *part, int parts, double *total, double *norm) {
+    const double acc = join_partials<P>(part, parts);
     if (threadIdx.x == 0) {
-        const double s = P == MBRL_NORM_TWO ? sqrt(acc) : acc;
-        *norm = s;
-        if (factor) {
-            const double c = max_norm / (s + 1e-6);
-            *factor = c > 1.0 ? 1.0 : c;
-        }
+        *total = acc;
+        *norm = root_of<P>(acc);
     }
 }
 
 // ---- clip ----
-// float32 values are multiplied in float64 and rounded once; 16-bit ones in float32, whose rounding of the factor is
-// 2^-16 of theirs.
-template <class E>
-__device__ __forceinline__ typename E::T scaled(typename E::T x, double c) {
-    using C = std::conditional_t<sizeof(typename E::T) == 2, float, double>;
-    return typename E::T(C(x) * C(c));
-}
+// Multiplies by the clipping factor in the type that the values are computed with: float32 for all but float64 ones, so the
+// factor is rounded (2^-24) and so is the product.  A factor below float32's normal range would lose digits: it is taken in
+// two, the second a power of 2.
+template <class C> struct Factor {
+    C first, second;
+    explicit __device__ __forceinline__ Factor(double c) {
+        const bool tiny = sizeof(C) == 4 && c < 0x1p-126;
+        first = C(tiny ? c * 0x1p64 : c);
+        second = C(tiny ? 0x1p-64 : 1.0);
+    }
+    __device__ __forceinline__ C operator()(C x) const { return x * first * second; }
+};
 
-template <class E>
-__device__ __forceinline__ void unit_scale(E, void *base, int64_t first, int n, double c) {
+template <bool kStream, class E>
+__device__ __forceinline__ void piece_scale(E, void *base, const Piece &p, double c) {
     using T = typename E::T;
     constexpr int V = E::V, kStep = kWave * V;
-    T *x = static_cast<T *>(base) + first;
-    const int lane = threadIdx.x % kWave;
+    T *x = static_cast<T *>(base) + p.first;
+    const Factor<typename E::C> f(c);
+    const int lane = threadIdx.x % kWave, n = p.n;
     int i = lane * V;
     for (; i + 3 * kStep + V <= n; i += 4 * kStep) {
         Pack<T, V> r[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) r[k] = load<T, V>(x + i + k * kStep);
+        for (int k = 0; k < 4; k++) r[k] = load<kStream, V>(x + i + k * kStep);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
 #pragma unroll
-            for (int j = 0; j < V; j++) r[k].v[j] = scaled<E>(r[k].v[j], c);
-            store<T, V>(x + i + k * kStep, r[k]);
+            for (int j = 0; j < V; j++) r[k].v[j] = T(f(r[k].v[j]));
+            store<kStream, V>(x + i + k * kStep, r[k]);
         }
     }
     for (; i + V <= n; i += kStep) {
-        Pack<T, V> r = load<T, V>(x + i);
+        Pack<T, V> r = load<kStream, V>(x + i);
 #pragma unroll
-        for (int j = 0; j < V; j++) r.v[j] = scaled<E>(r.v[j], c);
-        store<T, V>(x + i, r);
+        for (int j = 0; j < V; j++) r.v[j] = T(f(r.v[j]));
+        store<kStream, V>(x + i, r);
     }
     const int tail = n / V * V + lane;
-    if (tail < n) x[tail] = scaled<E>(x[tail], c);
+    if (tail < n) x[tail] = T(f(x[tail]));
 }
 
-__global__ __launch_bounds__(kThreads) void clip_scale(const NormList l, const double *factor) {
-    const double c = *factor;
-    if (c == 1.0) return;          // x * 1 is x: nothing to read or write
-    for (uint32_t unit = blockIdx.x * kWaves + wave_of_block(); unit < l.u.units; unit += gridDim.x * kWaves) {
-        const Piece p = piece(l.u, unit);
-        by_type(p.type, [&](auto e) { unit_scale(e, l.x[p.t], p.first, p.n, c); });
+// x * 1 is x: a factor of 1 leaves nothing to read or write.
+template <int P, bool kStream, class L>
+__global__ __launch_bounds__(kThreads) void clip_scale(const L l, const double *part, int parts, double max_norm, double *norm) {
+    const double s = root_of<P>(join_partials<P>(part, parts)), c = factor_of(s, max_norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = s;
+    if (c == 1.0) return;
+    dealt(l.u, wave_of_grid(), waves_of_grid(), [&](const Piece &p) {
+        by_type(p.type, [&](auto e) { piece_scale<kStream>(e, l.x[p.t], p, c); });
+    });
+}
+
+// A small list in one launch of one block.
+template <int P, bool kClip, class L>
+__global__ __launch_bounds__(kSmallThreads) void norm_small(const L l, double max_norm, double *norm) {
+    const double s = root_of<P>(small_norm<P>(l));
+    if (threadIdx.x == 0) *norm = s;
+    if constexpr (kClip) {
+        const double c = factor_of(s, max_norm);
+        if (c == 1.0) return;
+        shared_out(l.u, wave_of_block(), [&](const Piece &p) {
+            by_type(p.type, [&](auto e) { piece_scale<false>(e, l.x[p.t], p, c); });
+        });
     }
 }
 
 // ---- Adam ----
-// One thread a tensor: counts the step and turns it into what the update multiplies with, in float64.  A launch before the update, because every block of the update needs them.
-__global__ void adam_scalars(const StepList l, double b1, double b2, int decoupled, Scalars *out) {
-    const int i = threadIdx.x;
-    if (i >= l.count) return;
-    const float step = *l.step[i] + 1.0f;
-    *l.step[i] = step;
+struct Betas { double b1, b2, eps; };
+
+// Counts a tensor's step and turns it into what the update multiplies with, in float64.
+__device__ __forceinline__ Scalars count_step(float *count, double lr, double wd, const Betas &b, int decoupled) {
+    const float step = *count + 1.0f;
+    *count = step;
     const double t = step;
     Scalars s;
-    s.size = l.lr[i] / -expm1(t * log1p(b1 - 1.0));        // 1 - b^t without the cancellation (b - 1 is exact from 0.5 on)
-    s.root = 1.0 / sqrt(-expm1(t * log1p(b2 - 1.0)));
-    s.keep = decoupled ? 1.0 - l.lr[i] * l.wd[i] : 1.0;
-    s.l2 = decoupled ? 0.0 : l.wd[i];
-    out[i] = s;
+    s.size = lr / -expm1(t * log1p(b.b1 - 1.0));        // 1 - b^t without the cancellation (b - 1 is exact from 0.5 on)
+    s.root = 1.0 / sqrt(-expm1(t * log1p(b.b2 - 1.0)));
+    s.keep = decoupled ? 1.0 - lr * wd : 1.0;
+    s.l2 = decoupled ? 0.0 : wd;
+    return s;
 }
 
 // In float32 (float64 for float64 tensors); the state is float32 or wider, and a 16-bit parameter is rounded once, on
 // its way back.
 template <class C> struct Update {
-    C b1, a1, b2, a2, eps, clip, size, root, keep, l2;
+    C b1, a1, b2, a2, eps, size, root, keep, l2;
+    Factor<C> clip;
     __device__ __forceinline__ C operator()(C x, C g, C &m, C &v) const {
-        g = g * clip;
+        g = clip(g);
         if (l2 != C(0)) g = fma(l2, x, g);        // not 0 * x, which an infinite x makes NaN
         m = fma(b1, m, a1 * g);
         v = fma(b2, v, a2 * g * g);
@@ -263,45 +343,94 @@ template <class C> struct Update {
     }
 };
 
-struct Betas { double b1, b2, eps; };
-
-template <class E>
-__device__ __forceinline__ void unit_adam(E, void *pp, const void *gg, void *mm, void *vv, int64_t first, int n, const Betas &b,
-                                          const Scalars &s, double clip) {
+template <bool kStream, class E, class L>
+__device__ __forceinline__ void piece_adam(E, const L &l, const Piece &q, const Betas &b, const Scalars &s, double clip) {
     using T = typename E::T;
     using C = typename E::C;
     constexpr int V = sizeof(C) == 8 ? 2 : 4, kStep = kWave * V;
-    T *p = static_cast<T *>(pp) + first;
-    const T *g = static_cast<const T *>(gg) + first;
-    C *m = static_cast<C *>(mm) + first, *v = static_cast<C *>(vv) + first;
-    const Update<C> f{C(b.b1), C(1.0 - b.b1), C(b.b2), C(1.0 - b.b2), C(b.eps), C(clip), C(s.size), C(s.root), C(s.keep), C(s.l2)};
-    const int lane = threadIdx.x % kWave;
-    for (int i = lane * V; i + V <= n; i += kStep) {
-        Pack<T, V> rp = load<T, V>(p + i);
-        const Pack<T, V> rg = load<T, V>(g + i);
-        Pack<C, V> rm = load<C, V>(m + i), rv = load<C, V>(v + i);
+    T *p = static_cast<T *>(l.p[q.t]) + q.first;
+    const T *g = static_cast<const T *>(l.x[q.t]) + q.first;
+    C *m = static_cast<C *>(l.m[q.t]) + q.first, *v = static_cast<C *>(l.v[q.t]) + q.first;
+    const Update<C> f{C(b.b1), C(1.0 - b.b1), C(b.b2), C(1.0 - b.b2), C(b.eps), C(s.size), C(s.root), C(s.keep), C(s.l2), Factor<C>(clip)};
+    const int lane = threadIdx.x % kWave, n = q.n;
+    auto some = [&](int i, auto count) {        // `count` vectors a lane, all on their way at once
+        constexpr int N = count;
+        Pack<T, V> rp[N], rg[N];
+        Pack<C, V> rm[N], rv[N];
 #pragma unroll
-        for (int j = 0; j < V; j++) rp.v[j] = T(f(C(rp.v[j]), C(rg.v[j]), rm.v[j], rv.v[j]));
-        store<T, V>(p + i, rp);
-        store<C, V>(m + i, rm);
-        store<C, V>(v + i, rv);
-    }
+        for (int k = 0; k < N; k++) {
+            rg[k] = load<kStream, V>(g + i + k * kStep);
+            rm[k] = load<kStream, V>(m + i + k * kStep);
+            rv[k] = load<kStream, V>(v + i + k * kStep);
+            rp[k] = load<kStream, V>(p + i + k * kStep);
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+#pragma unroll
+            for (int j = 0; j < V; j++) rp[k].v[j] = T(f(C(rp[k].v[j]), C(rg[k].v[j]), rm[k].v[j], rv[k].v[j]));
+            store<kStream, V>(m + i + k * kStep, rm[k]);
+            store<kStream, V>(v + i + k * kStep, rv[k]);
+            store<kStream, V>(p + i + k * kStep, rp[k]);
+        }
+    };
+    int i = lane * V;
+    for (; i + kStep + V <= n; i += 2 * kStep) some(i, std::integral_constant<int, 2>{});
+    if (i + V <= n) some(i, std::integral_constant<int, 1>{});
     const int tail = n / V * V + lane;
     if (tail < n) p[tail] = T(f(C(p[tail]), C(g[tail]), m[tail], v[tail]));
 }
 
-__global__ __launch_bounds__(kThreads) void adam_update(const AdamList l, const Betas b, const Scalars *scalars, const double *factor) {
-    const double clip = factor ? *factor : 1.0;
-    for (uint32_t unit = blockIdx.x * kWaves + wave_of_block(); unit < l.u.units; unit += gridDim.x * kWaves) {
-        const Piece q = piece(l.u, unit);
-        const Scalars s = scalars[l.s[q.t]];
-        by_type(q.type, [&](auto e) { unit_adam(e, l.p[q.t], l.g[q.t], l.m[q.t], l.v[q.t], q.first, q.n, b, s, clip); });
+constexpr int kNoClip = -1;        // P of an update that does not clip
+
+// First launch of a step: the steps are counted (every block of the update needs what follows from them, so it cannot be
+// done there), and the gradients' partial sums made if they are to be clipped.
+template <int P, bool kStream, class L>
+__global__ __launch_bounds__(kThreads) void adam_begin(const L l, const Betas b, int decoupled, Scalars *scalars, double *part) {
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < l.u.count; i += kThreads) scalars[i] = count_step(l.step[i], l.lr[i], l.wd[i], b, decoupled);
+    if constexpr (P != kNoClip) {
+        const double acc = grid_norm<P, kStream>(l);
+        if (threadIdx.x == 0) part[blockIdx.x] = acc;
     }
 }
 
+template <int P, bool kStream, class L>
+__global__ __launch_bounds__(kThreads) void adam_update(const L l, const Betas b, const Scalars *scalars, const double *part, int parts,
+                                                        double max_norm, double *norm) {
+    double clip = 1.0;
+    if constexpr (P != kNoClip) {
+        const double s = root_of<P>(join_partials<P>(part, parts));
+        if (blockIdx.x == 0 && threadIdx.x == 0) *norm = s;
+        clip = factor_of(s, max_norm);
+    }
+    dealt(l.u, wave_of_grid(), waves_of_grid(), [&](const Piece &q) {
+        by_type(q.type, [&](auto e) { piece_adam<kStream>(e, l, q, b, scalars[q.t], clip); });
+    });
+}
+
+template <int P, class L>
+__global__ __launch_bounds__(kSmallThreads) void adam_small(const L a, const Betas b, int decoupled, double max_norm, double *norm) {
+    __shared__ Scalars scalars[decltype(a.l.u)::K];
+    static_assert(decltype(a.l.u)::K <= kWave, "one thread of one wave a tensor");
+    const int i = int(threadIdx.x) - (kSmallThreads - kWave);        // the last wave: where there is little to do, it has nothing else
+    if (i >= 0 && i < a.l.u.count) scalars[i] = count_step(a.step[i], a.lr[i], a.wd[i], b, decoupled);
+    double clip = 1.0;
+    if constexpr (P != kNoClip) {
+        const double s = root_of<P>(small_norm<P>(a.l));
+        if (threadIdx.x == 0) *norm = s;
+        clip = factor_of(s, max_norm);
+    }
+    __syncthreads();
+    shared_out(a.l.u, wave_of_block(), [&](const Piece &q) {
+        by_type(q.type, [&](auto e) { piece_adam<false>(e, a.l, q, b, scalars[q.t], clip); });
+    });
+}
+
 // ---- host ----
-// Values of a unit: small enough that the units of the list fill the chip's waves, large enough that finding a unit's
-// tensor does not count.
+const int kSize[4] = {8, 4, 2, 2};
+
+// How a list's values are cut and walked.  Small: one block.  Else up to kMaxBlocks blocks stay and take unit after unit,
+// with units small enough to fill them and large enough that finding a unit's tensor does not count.
 int unit_shift(int64_t values) {
     int shift = kMinShift;
     while (shift < kMaxShift && (values >> shift) > 4 * kMaxBlocks * kWaves) shift++;
@@ -314,33 +443,38 @@ int64_t total(int64_t count, const int64_t *numel) {
     return n;
 }
 
-// Runs through the tensors that have values, K at a time: fill(list, at, i) puts tensor i at place `at`, go(list, grid).
-template <int K, class List, class Fill, class Go>
-void in_lists(int64_t count, const int64_t *numel, const int *dtype, int shift, Fill fill, Go go) {
-    List l;
-    int at = 0;
+int64_t total_bytes(int64_t count, const int64_t *numel, const int *dtype) {
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; i++) n += numel[i] * kSize[dtype[i]];
+    return n;
+}
+
+// Puts tensors `from` to `to` of a call into a list: fill(list, place, tensor).  Empty ones have a place and no units.
+template <class List, class Fill>
+void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const int *dtype, int shift, Fill fill) {
     uint32_t units = 0;
-    auto flush = [&] {
-        if (!at) return;
-        l.u.count = at;
-        l.u.shift = shift;
-        l.u.units = units;
-        go(l, int(std::min<int64_t>((int64_t(units) + kWaves - 1) / kWaves, kMaxBlocks)));
-        at = 0;
-        units = 0;
-    };
-    for (int64_t i = 0; i < count; i++) {
-        if (!numel[i]) continue;
+    for (int64_t i = from; i < to; i++) {
+        const int at = int(i - from);
         units += uint32_t((numel[i] + (int64_t(1) << shift) - 1) >> shift);
         l.u.n[at] = uint64_t(numel[i]) << 2 | uint64_t(dtype[i]);
         l.u.end[at] = units;
-        fill(l, at, i);
-        if (++at == K) flush();
+        fill(at, i);
     }
-    flush();
+    l.u.count = int(to - from);
+    l.u.shift = shift;
+    l.u.units = units;
+}
+template <class U> int grid_of(const U &u, int most = kMaxBlocks) { return int(std::min<int64_t>((int64_t(u.units) + kWaves - 1) / kWaves, most)); }
+
+template <class F>
+void by_norm(int kind, F &&f) {
+    if (kind == MBRL_NORM_TWO) f(std::integral_constant<int, MBRL_NORM_TWO>{});
+    else if (kind == MBRL_NORM_ONE) f(std::integral_constant<int, MBRL_NORM_ONE>{});
+    else if (kind == MBRL_NORM_INF) f(std::integral_constant<int, MBRL_NORM_INF>{});
+    else f(std::integral_constant<int, kNoClip>{});
 }
 
-constexpr int64_t kMaxValues = int64_t(1) << 40;
+constexpr int64_t kMaxValues = int64_t(1) << 38;        // of a call: units are counted in 32 bits
 
 int check_list(const char *what, int64_t count, const int64_t *numel, const int *dtype) {
     static thread_local char text[160];
@@ -354,8 +488,6 @@ int check_list(const char *what, int64_t count, const int64_t *numel, const int 
     }
     return 0;
 }
-
-const int kSize[4] = {8, 4, 2, 2};
 
 // Memory that is written must not be any other memory of the call.
 struct Range { uintptr_t lo, hi; bool written; };
@@ -378,38 +510,73 @@ int launched(const char *what) {
     return report(-10, text);
 }
 
-int64_t partials(int64_t count) { return (count + kNormList - 1) / kNormList * kMaxBlocks; }
-
-// Workspace: [factor, unused][partial sums][Scalars of each tensor]
+// Workspace: [total, unused][partial sums][Scalars of each tensor]
+int64_t partials(int64_t count) { return (count + kAdamList - 1) / kAdamList * kMaxBlocks; }
 struct Space {
-    double *factor, *part;
+    double *total, *part;
     Scalars *scalars;
     Space(void *p, int64_t count) {
-        factor = static_cast<double *>(p);
-        part = factor + 2;
+        total = static_cast<double *>(p);
+        part = total + 2;
         scalars = reinterpret_cast<Scalars *>(part + partials(count));
     }
     static int64_t bytes(int64_t count) { return 16 + 8 * partials(count) + int64_t(sizeof(Scalars)) * count; }
 };
 
-template <int P>
-void launch_norm_as(int64_t count, const void *const *x, const int64_t *numel, const int *dtype, const Space &ws, double max_norm,
-                    double *norm, double *factor, hipStream_t st) {
-    int parts = 0;
-    in_lists<kNormList, NormList>(count, numel, dtype, unit_shift(total(count, numel)),
-        [&](NormList &l, int at, int64_t i) { l.x[at] = const_cast<void *>(x[i]); },
-        [&](const NormList &l, int grid) {
-            hipLaunchKernelGGL((norm_partials<P>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
-            parts += grid;
-        });
-    hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, max_norm, norm, factor);
-}
-
-void launch_norm(int kind, int64_t count, const void *const *x, const int64_t *numel, const int *dtype, const Space &ws, double max_norm,
-                 double *norm, double *factor, hipStream_t st) {
-    if (kind == MBRL_NORM_TWO) launch_norm_as<MBRL_NORM_TWO>(count, x, numel, dtype, ws, max_norm, norm, factor, st);
-    else if (kind == MBRL_NORM_ONE) launch_norm_as<MBRL_NORM_ONE>(count, x, numel, dtype, ws, max_norm, norm, factor, st);
-    else launch_norm_as<MBRL_NORM_INF>(count, x, numel, dtype, ws, max_norm, norm, factor, st);
+// The norm of a list, and the scaling where kClip.
+template <bool kClip>
+void launch_norm(int kind, int64_t count, void *const *x, const int64_t *numel, const int *dtype, const Space &ws, double max_norm,
+                 double *norm, hipStream_t st) {
+    const int64_t values = total(count, numel), bytes = total_bytes(count, numel, dtype);
+    by_norm(kind, [&](auto P_) {
+        constexpr int P = P_;
+        if constexpr (P != kNoClip) {
+            auto lists = [&](auto &l, int shift, auto go) {
+                constexpr int K = std::decay_t<decltype(l.u)>::K;
+                l.u.count = l.u.units = 0;
+                for (int64_t i = 0; i < count; i += K) {
+                    fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = x[k]; });
+                    go();
+                }
+            };
+            auto small = [&](auto l) {
+                lists(l, kSmallShift, [] {});
+                hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
+            };
+            auto large = [&](auto l, auto stream) {
+                constexpr bool kStream = stream;
+                using L = decltype(l);
+                const int shift = unit_shift(values);
+                int parts = 0;
+                lists(l, shift, [&] {
+                    if (const int grid = grid_of(l.u)) {
+                        hipLaunchKernelGGL((norm_partials<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
+                        parts += grid;
+                    }
+                });
+                const double *part = ws.part;
+                if (!kClip || kStream || parts > kMaxParts || !parts) {        // !parts: all tensors empty, no block below that would write the norm
+                    hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
+                    part = ws.total;
+                    parts = 1;
+                }
+                if constexpr (kClip)
+                    lists(l, kStream ? (bytes == 2 * values ? 11 : 10) : shift, [&] {
+                        if (const int grid = grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks))
+                            hipLaunchKernelGGL((clip_scale<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, part, parts, max_norm, norm);
+                    });
+            };
+            if (bytes <= (kClip ? kSmallClip : kSmallNorm) && count <= kNormList) {
+                if (count <= kFew) small(NormList<kFew>{});
+                else small(NormList<kNormList>{});
+            } else if (bytes > kCache) {
+                large(NormList<kNormList>{}, std::true_type{});
+            } else {
+                if (count <= kFew) large(NormList<kFew>{}, std::false_type{});
+                else large(NormList<kNormList>{}, std::false_type{});
+            }
+        }
+    });
 }
 
 template <class F>
@@ -440,7 +607,7 @@ int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel
         if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
             if (numel[i] && !grads[i]) return report(-1, "mbrl_grad_norm: null tensor");
-        launch_norm(norm_type, count, grads, numel, dtype, Space(workspace, count), 0.0, norm, nullptr, (hipStream_t)hip_stream);
+        launch_norm<false>(norm_type, count, const_cast<void *const *>(grads), numel, dtype, Space(workspace, count), 0.0, norm, (hipStream_t)hip_stream);
         return launched("mbrl_grad_norm");
     });
 }
@@ -462,12 +629,7 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
             r.push_back({lo, lo + uintptr_t(numel[i]) * kSize[dtype[i]], true});
         }
         if (!disjoint(r)) return report(-7, "mbrl_clip_grad_norm: two of the tensors share memory");
-        const hipStream_t st = (hipStream_t)hip_stream;
-        const Space ws(workspace, count);
-        launch_norm(norm_type, count, grads, numel, dtype, ws, max_norm, norm, ws.factor, st);
-        in_lists<kNormList, NormList>(count, numel, dtype, unit_shift(total(count, numel)),
-            [&](NormList &l, int at, int64_t i) { l.x[at] = grads[i]; },
-            [&](const NormList &l, int grid) { hipLaunchKernelGGL(clip_scale, dim3(grid), dim3(kThreads), 0, st, l, ws.factor); });
+        launch_norm<true>(norm_type, count, grads, numel, dtype, Space(workspace, count), max_norm, norm, (hipStream_t)hip_stream);
         return launched("mbrl_clip_grad_norm");
     });
 }
@@ -504,19 +666,59 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         if (!disjoint(r)) return report(-7, "mbrl_adam_step: a tensor that is written shares memory with another one");
         const hipStream_t st = (hipStream_t)hip_stream;
         const Space ws(workspace, count);
-        for (int64_t i = 0; i < count; i += kStepList) {
-            StepList l;
-            l.count = int(std::min<int64_t>(kStepList, count - i));
-            for (int k = 0; k < l.count; k++) l.step[k] = steps[i + k], l.lr[k] = lr[i + k], l.wd[k] = weight_decay[i + k];
-            hipLaunchKernelGGL(adam_scalars, dim3(1), dim3(kStepList), 0, st, l, beta_one, beta_two, decoupled, ws.scalars + i);
-        }
-        if (clip) launch_norm(norm_type, count, grads, numel, dtype, ws, max_norm, norm, ws.factor, st);
         const Betas b{beta_one, beta_two, eps};
-        in_lists<kAdamList, AdamList>(count, numel, dtype, unit_shift(total(count, numel)),
-            [&](AdamList &l, int at, int64_t i) { l.p[at] = params[i]; l.g[at] = grads[i]; l.m[at] = exp_avgs[i]; l.v[at] = exp_avg_sqs[i]; l.s[at] = uint32_t(i); },
-            [&](const AdamList &l, int grid) {
-                hipLaunchKernelGGL(adam_update, dim3(grid), dim3(kThreads), 0, st, l, b, ws.scalars, clip ? ws.factor : nullptr);
-            });
+        const int64_t values = total(count, numel);
+        int64_t bytes = 0;
+        for (int64_t i = 0; i < count; i++) bytes += numel[i] * (kSize[dtype[i]] == 8 ? 32 : 8 + 2 * kSize[dtype[i]]);
+        auto lists = [&](auto &l, int shift, auto fill, auto go) {
+            constexpr int K = std::decay_t<decltype(l.u)>::K;
+            l.u.count = l.u.units = 0;
+            for (int64_t i = 0; i < count; i += K) {
+                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = grads[k]; fill(at, k); });
+                go(i);
+            }
+        };
+        auto tensors = [&](auto &l) { return [&](int at, int64_t k) { l.p[at] = params[k]; l.m[at] = exp_avgs[k]; l.v[at] = exp_avg_sqs[k]; }; };
+        auto counters = [&](auto &l) { return [&](int at, int64_t k) { l.step[at] = steps[k]; l.lr[at] = lr[k]; l.wd[at] = weight_decay[k]; }; };
+        by_norm(clip ? norm_type : kNoClip, [&](auto P_) {
+            constexpr int P = P_;
+            auto small = [&](auto l) {
+                lists(l.l, kSmallShift, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
+                hipLaunchKernelGGL((adam_small<P, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, b, decoupled, max_norm, norm);
+            };
+            auto large = [&](auto begin, auto update, auto stream) {
+                constexpr bool kStream = stream;
+                const int shift = unit_shift(values);
+                int parts = 0;
+                lists(begin, shift, counters(begin), [&](int64_t i) {
+                    const int grid = clip ? std::max(grid_of(begin.u), 1) : 1;
+                    hipLaunchKernelGGL((adam_begin<P, kStream, decltype(begin)>), dim3(grid), dim3(kThreads), 0, st, begin, b, decoupled,
+                                       ws.scalars + i, ws.part + parts);
+                    parts += grid;
+                });
+                const double *part = ws.part;
+                if constexpr (P != kNoClip)
+                    if (kStream || parts > kMaxParts) {
+                        hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
+                        part = ws.total;
+                        parts = 1;
+                    }
+                lists(update, kStream ? 8 : shift, tensors(update), [&](int64_t i) {
+                    if (const int grid = std::max(grid_of(update.u, kStream ? kStreamBlocks : kMaxBlocks), clip && i == 0 ? 1 : 0))        // one block at least writes the norm
+                        hipLaunchKernelGGL((adam_update<P, kStream, decltype(update)>), dim3(grid), dim3(kThreads), 0, st, update, b,
+                                           ws.scalars + i, part, parts, max_norm, norm);
+                });
+            };
+            if (bytes <= kSmallAdam && count <= kStepList) {
+                if (count <= kFew) small(StepList<kFew>{});
+                else small(StepList<kStepList>{});
+            } else if (bytes > kCache) {
+                large(BeginList<kAdamList>{}, UpdateList<kAdamList>{}, std::true_type{});
+            } else {
+                if (count <= kFew) large(BeginList<kFew>{}, UpdateList<kFew>{}, std::false_type{});
+                else large(BeginList<kAdamList>{}, UpdateList<kAdamList>{}, std::false_type{});
+            }
+        });
         return launched("mbrl_adam_step");
     });
 }
