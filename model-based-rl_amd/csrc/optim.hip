@@ -32,6 +32,7 @@ using mbrl::report;
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMaxBlocks = 1024;          // of a launch: 4 blocks of 4 waves a CU
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
+constexpr int kUnits = 2;                 // units of a wave, at least, where waves stay
 constexpr int kMinShift = 9, kMaxShift = 12, kSmallShift = 8;
 constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;      // bytes that one block takes on alone
 constexpr int kMaxParts = 2048;           // partial sums that every block of a second launch joins for itself
@@ -82,15 +83,18 @@ template <int K_> struct Units {
 template <int K> struct NormList { Units<K> u; void *x[K]; };
 template <int K> struct BeginList { Units<K> u; const void *x[K]; float *step[K]; double lr[K], wd[K]; };       // x: gradients
 template <int K> struct UpdateList { Units<K> u; const void *x[K]; void *p[K], *m[K], *v[K]; };
-template <int K> struct StepList { UpdateList<K> l; float *step[K]; double lr[K], wd[K]; };                     // both, for one launch
-constexpr int kFew = 16, kNormList = 192, kAdamList = 80, kStepList = 52;
+template <int K> struct SmallList { UpdateList<K> l; float *step[K]; double lr[K], wd[K]; };                    // both, for one launch
+template <int K> struct CountList { float *step[K]; double lr[K], wd[K]; int count; };
+constexpr int kFew = 16, kNormList = 192, kAdamList = 80, kSmallList = 52, kCountList = 160;
 static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kAdamList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
-              sizeof(StepList<kStepList>) <= 3968, "kernel arguments are 4 KB");
+              sizeof(SmallList<kSmallList>) <= 3968 && sizeof(CountList<kCountList>) <= 3968, "kernel arguments are 4 KB");
 
 // What the update of one tensor multiplies with.
 struct Scalars { double size, root, keep, l2; };
 
 __device__ __forceinline__ uint32_t wave_of_block() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+__device__ __forceinline__ uint32_t wave_of_grid() { return blockIdx.x * kWaves + wave_of_block(); }
+__device__ __forceinline__ uint32_t waves_of_grid() { return gridDim.x * kWaves; }
 
 // The tensor that unit `unit` belongs to: as many as end at or before it come first.
 template <class U>
@@ -127,11 +131,16 @@ __device__ __forceinline__ void dealt(const U &u, uint32_t wave, uint32_t waves,
         f(piece(u, unit, unit + 1));
     }
 }
-// The same for the waves of one block: units one after another, so that each has few tensors to find.
+// The same, but units one after another, so that a wave has few tensors to find.
 template <class U, class F>
-__device__ __forceinline__ void shared_out(const U &u, uint32_t wave, F f) {
-    const uint32_t each = (u.units + kSmallWaves - 1) / kSmallWaves, stop = min(u.units, (wave + 1) * each);
+__device__ __forceinline__ void shared_out(const U &u, uint32_t wave, uint32_t waves, F f) {
+    const uint32_t each = (u.units + waves - 1) / waves, stop = min(u.units, (wave + 1) * each);
     for (uint32_t unit = wave * each; unit < stop;) f(piece(u, unit, stop));
+}
+template <bool kStream, class U, class F>
+__device__ __forceinline__ void walk(const U &u, F f) {
+    if constexpr (kStream) dealt(u, wave_of_grid(), waves_of_grid(), f);
+    else shared_out(u, wave_of_grid(), waves_of_grid(), f);
 }
 
 // ---- norm ----
@@ -192,13 +201,11 @@ __device__ __forceinline__ double piece_norm(E, const void *base, const Piece &p
     return join<P>(a[0], a[1]);
 }
 
-__device__ __forceinline__ uint32_t wave_of_grid() { return blockIdx.x * kWaves + wave_of_block(); }
-__device__ __forceinline__ uint32_t waves_of_grid() { return gridDim.x * kWaves; }
 
 template <int P, bool kStream, class L>
 __device__ __forceinline__ double grid_norm(const L &l) {
     double acc = 0.0;
-    dealt(l.u, wave_of_grid(), waves_of_grid(), [&](const Piece &p) {
+    walk<kStream>(l.u, [&](const Piece &p) {
         by_type(p.type, [&](auto e) { acc = piece_norm<P, kStream>(e, l.x[p.t], p, acc); });
     });
     return block_join<P, kWaves>(acc);
@@ -206,7 +213,7 @@ __device__ __forceinline__ double grid_norm(const L &l) {
 template <int P, class L>
 __device__ __forceinline__ double small_norm(const L &l) {
     double acc = 0.0;
-    shared_out(l.u, wave_of_block(), [&](const Piece &p) {
+    shared_out(l.u, wave_of_block(), kSmallWaves, [&](const Piece &p) {
         by_type(p.type, [&](auto e) { acc = piece_norm<P, false>(e, l.x[p.t], p, acc); });
     });
     return block_join<P, kSmallWaves>(acc);
@@ -293,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void clip_scale(const L l, const double *
     const double s = root_of<P>(join_partials<P>(part, parts)), c = factor_of(s, max_norm);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = s;
     if (c == 1.0) return;
-    dealt(l.u, wave_of_grid(), waves_of_grid(), [&](const Piece &p) {
+    walk<kStream>(l.u, [&](const Piece &p) {
         by_type(p.type, [&](auto e) { piece_scale<kStream>(e, l.x[p.t], p, c); });
     });
 }
@@ -306,14 +313,14 @@ __global__ __launch_bounds__(kSmallThreads) void norm_small(const L l, double ma
     if constexpr (kClip) {
         const double c = factor_of(s, max_norm);
         if (c == 1.0) return;
-        shared_out(l.u, wave_of_block(), [&](const Piece &p) {
+        shared_out(l.u, wave_of_block(), kSmallWaves, [&](const Piece &p) {
             by_type(p.type, [&](auto e) { piece_scale<false>(e, l.x[p.t], p, c); });
         });
     }
 }
 
 // ---- Adam ----
-struct Betas { double b1, b2, eps; };
+struct Betas { double b1, b2, log_b1, log_b2, eps; };
 
 // Counts a tensor's step and turns it into what the update multiplies with, in float64.
 __device__ __forceinline__ Scalars count_step(float *count, double lr, double wd, const Betas &b, int decoupled) {
@@ -321,8 +328,8 @@ __device__ __forceinline__ Scalars count_step(float *count, double lr, double wd
     *count = step;
     const double t = step;
     Scalars s;
-    s.size = lr / -expm1(t * log1p(b.b1 - 1.0));        // 1 - b^t without the cancellation (b - 1 is exact from 0.5 on)
-    s.root = 1.0 / sqrt(-expm1(t * log1p(b.b2 - 1.0)));
+    s.size = lr / -expm1(t * b.log_b1);        // 1 - b^t without the cancellation
+    s.root = 1.0 / sqrt(-expm1(t * b.log_b2));
     s.keep = decoupled ? 1.0 - lr * wd : 1.0;
     s.l2 = decoupled ? 0.0 : wd;
     return s;
@@ -394,6 +401,12 @@ __global__ __launch_bounds__(kThreads) void adam_begin(const L l, const Betas b,
     }
 }
 
+// For lists too long for that: the steps apart, the norm as of any list.
+__global__ __launch_bounds__(kCountList) void adam_count(const CountList<kCountList> l, const Betas b, int decoupled, Scalars *scalars) {
+    const int i = threadIdx.x;
+    if (i < l.count) scalars[i] = count_step(l.step[i], l.lr[i], l.wd[i], b, decoupled);
+}
+
 template <int P, bool kStream, class L>
 __global__ __launch_bounds__(kThreads) void adam_update(const L l, const Betas b, const Scalars *scalars, const double *part, int parts,
                                                         double max_norm, double *norm) {
@@ -421,7 +434,7 @@ __global__ __launch_bounds__(kSmallThreads) void adam_small(const L a, const Bet
         clip = factor_of(s, max_norm);
     }
     __syncthreads();
-    shared_out(a.l.u, wave_of_block(), [&](const Piece &q) {
+    shared_out(a.l.u, wave_of_block(), kSmallWaves, [&](const Piece &q) {
         by_type(q.type, [&](auto e) { piece_adam<false>(e, a.l, q, b, scalars[q.t], clip); });
     });
 }
@@ -464,7 +477,9 @@ void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const in
     l.u.shift = shift;
     l.u.units = units;
 }
-template <class U> int grid_of(const U &u, int most = kMaxBlocks) { return int(std::min<int64_t>((int64_t(u.units) + kWaves - 1) / kWaves, most)); }
+template <class U> int grid_of(const U &u, int most = kMaxBlocks, int each = 1) {
+    return int(std::min<int64_t>((int64_t(u.units) + kWaves * each - 1) / (kWaves * each), most));
+}
 
 template <class F>
 void by_norm(int kind, F &&f) {
@@ -490,17 +505,34 @@ int check_list(const char *what, int64_t count, const int64_t *numel, const int 
 }
 
 // Memory that is written must not be any other memory of the call.
-struct Range { uintptr_t lo, hi; bool written; };
-bool disjoint(std::vector<Range> &r) {
-    std::sort(r.begin(), r.end(), [](const Range &a, const Range &b) { return a.lo < b.lo; });
-    uintptr_t read_end = 0, write_end = 0;
-    for (const Range &x : r) {
-        if (x.lo < write_end || (x.written && x.lo < read_end)) return false;
-        uintptr_t &end = x.written ? write_end : read_end;
-        end = std::max(end, x.hi);
+struct Ranges {
+    struct Range { uintptr_t lo, hi; bool written; };
+    std::vector<Range> r;
+    void add(const void *p, int64_t bytes, bool written) {
+        if (bytes) r.push_back({uintptr_t(p), uintptr_t(p) + uintptr_t(bytes), written});
     }
-    return true;
-}
+    bool disjoint() const {
+        // Device addresses have 48 bits: with the place behind them they are sorted as plain numbers, four times as fast
+        // as the ranges themselves (900 of them: 8 us for 34), which a long list's step would wait for.
+        std::vector<uint64_t> order;
+        order.reserve(r.size());
+        uintptr_t read_end = 0, write_end = 0;
+        auto next = [&](const Range &x) {
+            if (x.lo < write_end || (x.written && x.lo < read_end)) return false;
+            uintptr_t &end = x.written ? write_end : read_end;
+            end = std::max(end, x.hi);
+            return true;
+        };
+        bool packed = r.size() <= 0x10000;
+        for (const Range &x : r) packed = packed && x.lo < (uintptr_t(1) << 48);
+        for (size_t i = 0; i < r.size(); i++) order.push_back(packed ? uint64_t(r[i].lo) << 16 | i : i);
+        if (packed) std::sort(order.begin(), order.end());
+        else std::sort(order.begin(), order.end(), [&](uint64_t a, uint64_t b) { return r[a].lo < r[b].lo; });
+        for (uint64_t i : order)
+            if (!next(r[packed ? i & 0xffff : i])) return false;
+        return true;
+    }
+};
 
 int launched(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -511,7 +543,7 @@ int launched(const char *what) {
 }
 
 // Workspace: [total, unused][partial sums][Scalars of each tensor]
-int64_t partials(int64_t count) { return (count + kAdamList - 1) / kAdamList * kMaxBlocks; }
+int64_t partials(int64_t count) { return (count + kNormList - 1) / kNormList * kMaxBlocks; }
 struct Space {
     double *total, *part;
     Scalars *scalars;
@@ -523,37 +555,73 @@ struct Space {
     static int64_t bytes(int64_t count) { return 16 + 8 * partials(count) + int64_t(sizeof(Scalars)) * count; }
 };
 
+// The gradients of a call, for a norm or scaling, to which it is all one where a tensor ends: neighbours in memory of one type
+// become one.  A bucket of many tensors is one long run then, which takes one launch instead of one for each kNormList.
+struct Gradients {
+    int64_t count, values, bytes;
+    void *const *x;
+    const int64_t *numel;
+    const int *dtype;
+    std::vector<void *> x_;
+    std::vector<int64_t> numel_;
+    std::vector<int> dtype_;
+
+    Gradients(int64_t count_, void *const *xs, const int64_t *ns, const int *types)
+        : count(count_), values(total(count_, ns)), bytes(total_bytes(count_, ns, types)), x(xs), numel(ns), dtype(types) {
+        auto follows = [&](int64_t i) {
+            return types[i] == types[i - 1] && ns[i - 1] && static_cast<char *>(xs[i - 1]) + ns[i - 1] * kSize[types[i]] == xs[i];
+        };
+        int64_t runs = count ? 1 : 0;
+        for (int64_t i = 1; i < count; i++) runs += !follows(i);
+        if (runs == count) return;
+        x_.reserve(runs), numel_.reserve(runs), dtype_.reserve(runs);
+        for (int64_t i = 0; i < count; i++) {
+            if (i && follows(i)) {
+                numel_.back() += ns[i];
+                continue;
+            }
+            x_.push_back(xs[i]), numel_.push_back(ns[i]), dtype_.push_back(types[i]);
+        }
+        count = runs;
+        x = x_.data(), numel = numel_.data(), dtype = dtype_.data();
+    }
+
+    template <class L, class Go> void lists(L &l, int shift, Go go) const {
+        constexpr int K = decltype(l.u)::K;
+        l.u.count = l.u.units = 0;
+        for (int64_t i = 0; i < count; i += K) {
+            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = x[k]; });
+            go();
+        }
+    }
+};
+
+// -> how many partial sums there are
+template <int P, bool kStream, class L>
+int launch_partials(L &l, const Gradients &g, double *part, hipStream_t st) {
+    int parts = 0;
+    g.lists(l, unit_shift(g.values), [&] {
+        if (const int grid = grid_of(l.u, kMaxBlocks, kStream ? 1 : kUnits)) {
+            hipLaunchKernelGGL((norm_partials<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, part + parts);
+            parts += grid;
+        }
+    });
+    return parts;
+}
+
 // The norm of a list, and the scaling where kClip.
 template <bool kClip>
-void launch_norm(int kind, int64_t count, void *const *x, const int64_t *numel, const int *dtype, const Space &ws, double max_norm,
-                 double *norm, hipStream_t st) {
-    const int64_t values = total(count, numel), bytes = total_bytes(count, numel, dtype);
+void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm, double *norm, hipStream_t st) {
     by_norm(kind, [&](auto P_) {
         constexpr int P = P_;
         if constexpr (P != kNoClip) {
-            auto lists = [&](auto &l, int shift, auto go) {
-                constexpr int K = std::decay_t<decltype(l.u)>::K;
-                l.u.count = l.u.units = 0;
-                for (int64_t i = 0; i < count; i += K) {
-                    fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = x[k]; });
-                    go();
-                }
-            };
             auto small = [&](auto l) {
-                lists(l, kSmallShift, [] {});
+                g.lists(l, kSmallShift, [] {});
                 hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
             };
             auto large = [&](auto l, auto stream) {
                 constexpr bool kStream = stream;
-                using L = decltype(l);
-                const int shift = unit_shift(values);
-                int parts = 0;
-                lists(l, shift, [&] {
-                    if (const int grid = grid_of(l.u)) {
-                        hipLaunchKernelGGL((norm_partials<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
-                        parts += grid;
-                    }
-                });
+                int parts = launch_partials<P, kStream>(l, g, ws.part, st);
                 const double *part = ws.part;
                 if (!kClip || kStream || parts > kMaxParts || !parts) {        // !parts: all tensors empty, no block below that would write the norm
                     hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
@@ -561,18 +629,18 @@ void launch_norm(int kind, int64_t count, void *const *x, const int64_t *numel, 
                     parts = 1;
                 }
                 if constexpr (kClip)
-                    lists(l, kStream ? (bytes == 2 * values ? 11 : 10) : shift, [&] {
-                        if (const int grid = grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks))
-                            hipLaunchKernelGGL((clip_scale<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, part, parts, max_norm, norm);
+                    g.lists(l, kStream ? (g.bytes == 2 * g.values ? 11 : 10) : unit_shift(g.values), [&] {
+                        if (const int grid = kStream ? grid_of(l.u, kStreamBlocks) : grid_of(l.u, kMaxBlocks, kUnits))
+                            hipLaunchKernelGGL((clip_scale<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, part, parts, max_norm, norm);
                     });
             };
-            if (bytes <= (kClip ? kSmallClip : kSmallNorm) && count <= kNormList) {
-                if (count <= kFew) small(NormList<kFew>{});
+            if (g.bytes <= (kClip ? kSmallClip : kSmallNorm) && g.count <= kNormList) {
+                if (g.count <= kFew) small(NormList<kFew>{});
                 else small(NormList<kNormList>{});
-            } else if (bytes > kCache) {
+            } else if (g.bytes > kCache) {
                 large(NormList<kNormList>{}, std::true_type{});
             } else {
-                if (count <= kFew) large(NormList<kFew>{}, std::false_type{});
+                if (g.count <= kFew) large(NormList<kFew>{}, std::false_type{});
                 else large(NormList<kNormList>{}, std::false_type{});
             }
         }
@@ -607,7 +675,8 @@ int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel
         if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
             if (numel[i] && !grads[i]) return report(-1, "mbrl_grad_norm: null tensor");
-        launch_norm<false>(norm_type, count, const_cast<void *const *>(grads), numel, dtype, Space(workspace, count), 0.0, norm, (hipStream_t)hip_stream);
+        launch_norm<false>(norm_type, Gradients(count, const_cast<void *const *>(grads), numel, dtype), Space(workspace, count), 0.0, norm,
+                           (hipStream_t)hip_stream);
         return launched("mbrl_grad_norm");
     });
 }
@@ -620,16 +689,14 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
         if (!(max_norm >= 0.0)) return report(-7, "mbrl_clip_grad_norm: max_norm must not be negative");
         if (!norm || !workspace || (count && !grads)) return report(-1, "mbrl_clip_grad_norm: null argument");
         if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_clip_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
-        std::vector<Range> r;
-        r.reserve(count);
+        Ranges r;
+        r.r.reserve(count);
         for (int64_t i = 0; i < count; i++) {
-            if (!numel[i]) continue;
-            if (!grads[i]) return report(-1, "mbrl_clip_grad_norm: null tensor");
-            const uintptr_t lo = uintptr_t(grads[i]);
-            r.push_back({lo, lo + uintptr_t(numel[i]) * kSize[dtype[i]], true});
+            if (numel[i] && !grads[i]) return report(-1, "mbrl_clip_grad_norm: null tensor");
+            r.add(grads[i], numel[i] * kSize[dtype[i]], true);
         }
-        if (!disjoint(r)) return report(-7, "mbrl_clip_grad_norm: two of the tensors share memory");
-        launch_norm<true>(norm_type, count, grads, numel, dtype, Space(workspace, count), max_norm, norm, (hipStream_t)hip_stream);
+        if (!r.disjoint()) return report(-7, "mbrl_clip_grad_norm: two of the tensors share memory");
+        launch_norm<true>(norm_type, Gradients(count, grads, numel, dtype), Space(workspace, count), max_norm, norm, (hipStream_t)hip_stream);
         return launched("mbrl_clip_grad_norm");
     });
 }
@@ -648,25 +715,25 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         if (!workspace || (count && (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps || !lr || !weight_decay)))
             return report(-1, "mbrl_adam_step: null argument");
         if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_adam_step: workspace too small (mbrl_optim_workspace_bytes)");
-        std::vector<Range> r;
-        r.reserve(5 * count);
-        for (int64_t i = 0; i < count; i++) {
+        for (int64_t i = 0; i < count; i++)
             if (!steps[i] || (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i])))
                 return report(-1, "mbrl_adam_step: null tensor");
-            const int64_t size = kSize[dtype[i]], wide = size == 8 ? 8 : 4;
-            auto range = [&](const void *p, int64_t bytes, bool written) {
-                if (bytes) r.push_back({uintptr_t(p), uintptr_t(p) + uintptr_t(bytes), written});
-            };
-            range(params[i], numel[i] * size, true);
-            range(grads[i], numel[i] * size, false);
-            range(exp_avgs[i], numel[i] * wide, true);
-            range(exp_avg_sqs[i], numel[i] * wide, true);
-            range(steps[i], 4, true);
-        }
-        if (!disjoint(r)) return report(-7, "mbrl_adam_step: a tensor that is written shares memory with another one");
+        Ranges r;
+        r.r.reserve(5 * count);
+        auto add = [&](auto x, bool written, auto bytes) {
+            for (int64_t i = 0; i < count; i++) r.add(x[i], bytes(i), written);
+        };
+        auto own = [&](int64_t i) { return numel[i] * kSize[dtype[i]]; };
+        auto wide = [&](int64_t i) { return numel[i] * (kSize[dtype[i]] == 8 ? 8 : 4); };
+        add(params, true, own);
+        add(grads, false, own);
+        add(exp_avgs, true, wide);
+        add(exp_avg_sqs, true, wide);
+        add(steps, true, [](int64_t) { return 4; });
+        if (!r.disjoint()) return report(-7, "mbrl_adam_step: a tensor that is written shares memory with another one");
         const hipStream_t st = (hipStream_t)hip_stream;
         const Space ws(workspace, count);
-        const Betas b{beta_one, beta_two, eps};
+        const Betas b{beta_one, beta_two, std::log1p(beta_one - 1.0), std::log1p(beta_two - 1.0), eps};        // b - 1 is exact from 0.5 on
         const int64_t values = total(count, numel);
         int64_t bytes = 0;
         for (int64_t i = 0; i < count; i++) bytes += numel[i] * (kSize[dtype[i]] == 8 ? 32 : 8 + 2 * kSize[dtype[i]]);
@@ -690,12 +757,30 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
                 constexpr bool kStream = stream;
                 const int shift = unit_shift(values);
                 int parts = 0;
-                lists(begin, shift, counters(begin), [&](int64_t i) {
-                    const int grid = clip ? std::max(grid_of(begin.u), 1) : 1;
-                    hipLaunchKernelGGL((adam_begin<P, kStream, decltype(begin)>), dim3(grid), dim3(kThreads), 0, st, begin, b, decoupled,
-                                       ws.scalars + i, ws.part + parts);
-                    parts += grid;
-                });
+                if (count <= kAdamList) {
+                    lists(begin, shift, counters(begin), [&](int64_t) {
+                        parts = clip ? std::max(grid_of(begin.u), 1) : 1;
+                        hipLaunchKernelGGL((adam_begin<P, kStream, decltype(begin)>), dim3(parts), dim3(kThreads), 0, st, begin, b, decoupled,
+                                           ws.scalars, ws.part);
+                    });
+                } else {
+                    CountList<kCountList> l;
+                    for (int64_t i = 0; i < count; i += kCountList) {
+                        l.count = int(std::min<int64_t>(count - i, kCountList));
+                        for (int k = 0; k < l.count; k++) counters(l)(k, i + k);
+                        hipLaunchKernelGGL(adam_count, dim3(1), dim3(kCountList), 0, st, l, b, decoupled, ws.scalars + i);
+                    }
+                    if constexpr (P != kNoClip) {
+                        const Gradients g(count, const_cast<void *const *>(grads), numel, dtype);
+                        if (g.count <= kFew && !kStream) {
+                            NormList<kFew> few;
+                            parts = launch_partials<P, false>(few, g, ws.part, st);
+                        } else {
+                            NormList<kNormList> many;
+                            parts = launch_partials<P, kStream>(many, g, ws.part, st);
+                        }
+                    }
+                }
                 const double *part = ws.part;
                 if constexpr (P != kNoClip)
                     if (kStream || parts > kMaxParts) {
@@ -709,9 +794,9 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
                                            ws.scalars + i, part, parts, max_norm, norm);
                 });
             };
-            if (bytes <= kSmallAdam && count <= kStepList) {
-                if (count <= kFew) small(StepList<kFew>{});
-                else small(StepList<kStepList>{});
+            if (bytes <= kSmallAdam && count <= kSmallList) {
+                if (count <= kFew) small(SmallList<kFew>{});
+                else small(SmallList<kSmallList>{});
             } else if (bytes > kCache) {
                 large(BeginList<kAdamList>{}, UpdateList<kAdamList>{}, std::true_type{});
             } else {

@@ -410,6 +410,89 @@ def test_streams_beside_each_other():
         assert abs(float(n[1]) - 1.0) < 2e-6 and float(n[2]) <= 1.0 + 2.0 ** -24
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_neighbours_in_one_buffer(dtype):
+    """Tensors that follow each other in memory, empty ones and another type between them, and a gap: every value once."""
+    torch, optim = _t()
+    sizes = [700, 1, 0, 0, 63, 4097, 512, 0, 9, 30000]
+    whole = make([(sum(sizes) + 5,)], [dtype], seed=71)[0]
+    parts = list(whole[:sum(sizes)].split(sizes))
+    other = make([(333,)], ["float32" if dtype != "float32" else "float64"], seed=72)[0]
+    ts = parts[:4] + [other] + parts[4:8] + parts[9:]           # parts[8] is left out
+    for p in (2.0, math.inf):
+        arrays = host(ts)
+        assert abs(float(optim.grad_norm(ts, p)) - ref_norm(arrays, p)) <= norm_tol(arrays) * ref_norm(arrays, p)
+        assert float(optim.grad_norm(ts[::-1], p)) == pytest.approx(ref_norm(arrays, p), rel=1e-12)
+    keep = whole.clone()
+    optim.clip_grad_norm_(ts, 0.0)
+    at = sum(sizes[:8])
+    assert torch.equal(whole[at:at + 9], keep[at:at + 9]) and torch.equal(whole[sum(sizes):], keep[sum(sizes):])
+    assert not any(bool(t.any()) for t in ts)
+
+
+@pytest.mark.parametrize("dtype,n", [("float32", 69_000_001), ("bfloat16", 138_000_003), ("float16", 138_000_003), ("float64", 35_000_001)])
+def test_lists_beyond_the_cache(dtype, n):
+    """More than 256 MB, where the accesses and the walk are others; expected values in float64 on the device."""
+    torch, optim = _t()
+    kind = getattr(torch, dtype)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    # two tensors of one odd buffer (one run to the norm) and a small one apart
+    whole = torch.randn(n + 1, dtype=torch.float32, device="cuda", generator=g).to(kind)[1:]
+    ts = [whole[:n // 3], whole[n // 3:], torch.randn(77, dtype=torch.float32, device="cuda", generator=g).to(kind)]
+    total = sum(float(t.double().square().sum()) for t in ts)
+    want = math.sqrt(total)
+    tol = (n + 81) * 2.0 ** -53
+    assert abs(float(optim.grad_norm(ts)) - want) <= tol * want
+    assert float(optim.grad_norm(ts, math.inf)) == max(float(t.abs().max()) for t in ts)
+    keep = [t.clone() for t in ts]
+    norm = optim.clip_grad_norm_(ts, 2 * want)
+    assert all(torch.equal(a, b) for a, b in zip(ts, keep))
+    norm = optim.clip_grad_norm_(ts, 0.3 * want)
+    c = 0.3 * want / (float(norm) + 1e-6)
+    rel = HALF[dtype] + 4 * 2.0 ** -53 + {"float64": 0.0, "float32": 2.0 ** -24}.get(dtype, 2 * 2.0 ** -24)
+    for t, k in zip(ts, keep):
+        e = k.double() * c
+        assert bool(((t.double() - e).abs() <= 1.001 * rel * e.abs() + TINY[dtype]).all())
+
+
+@pytest.mark.parametrize("dtype,n", [("float32", 17_000_001), ("bfloat16", 23_000_003), ("float64", 9_000_001)])
+@pytest.mark.parametrize("most", [None, 0.3])
+@pytest.mark.parametrize("parts", [3, 90])
+def test_adam_beyond_the_cache(dtype, n, most, parts):
+    """The same of the update, for 3 tensors and for more than one launch takes."""
+    torch, optim = _t()
+    kind, wide = getattr(torch, dtype), torch.float64 if dtype == "float64" else torch.float32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    new = lambda k: torch.randn(n, dtype=torch.float32, device="cuda", generator=g).to(k)      # noqa: E731
+    p, x, m, v = new(kind), new(kind), new(wide), new(wide).square_()
+    cut = lambda t: list(t.tensor_split(parts))       # noqa: E731
+    q, a, b = p.clone(), m.clone(), v.clone()
+    norm = optim.adam_step(cut(q), cut(x), cut(a), cut(b), [torch.ones((), device="cuda") for _ in range(parts)], 0.01, weight_decay=0.1,
+                           max_norm=None if most is None else most * math.sqrt(n))
+    c = 1.0
+    if most is not None:
+        want = float(x.double().square().sum()) ** 0.5
+        assert abs(float(norm) - want) <= (n + 4) * 2.0 ** -53 * want
+        c = most * math.sqrt(n) / (float(norm) + 1e-6)
+    u, w = HALF["float64" if dtype == "float64" else "float32"], 2.0 ** -53
+    for s in torch.arange(n, device="cuda").tensor_split(8):
+        lo, hi = int(s[0]), int(s[-1]) + 1
+        X, G, M, V = (t[lo:hi].double() for t in (p, x, m, v))
+        G = c * G + 0.1 * X
+        M1, V1 = 0.9 * M + 0.1 * G, 0.999 * V + 0.001 * G * G
+        d = V1.sqrt() / math.sqrt(1 - 0.999 ** 2) + 1e-8
+        X1 = X - 0.01 / (1 - 0.9 ** 2) * M1 / d
+        # adam_bounds(), its terms rounded up: 8 u of each summand of m', 12 u of v', 24 u of the update's parts; the factor
+        # 1 - 0.999^2 written as here is off by 2^-53 / 0.002 = 500 w
+        em = 8 * u * (0.9 * M.abs() + 0.1 * (c * x[lo:hi].double().abs() + 0.2 * X.abs()))
+        ev = 12 * u * (V1 + 0.002 * (c * x[lo:hi].double().abs() + 0.1 * X.abs()).square())
+        ex = 0.0527 * (em + (24 * u + 600 * w) * M1.abs() + M1.abs() * ev / V1) / d + 2 * u * X1.abs() + (HALF[dtype] if kind != wide else 0.0) * X1.abs() * 1.01
+        for got, ref, e in ((q, X1, ex), (a, M1, em), (b, V1, ev)):
+            assert bool(((got[lo:hi].double() - ref).abs() <= e + 1e-37).all())
+
+
 def test_more_values_than_32_bits_count():
     """One float16 tensor of 2^31 + 4099 values (4 GiB): the last ones count, and are reached."""
     torch, optim = _t()

@@ -112,6 +112,11 @@ def test_abi_refusals():
     assert adam(steps=None) == -1 and adam(grads=None) == -1
     for over in (dict(avgs=0x10000), dict(sqs=0x30000), dict(grads=0x10020), dict(steps=0x40004)):
         assert adam(**over) == -7 and b"shares memory" in L.mbrl_last_error(), over
+    # also in a list too long for the short sort: 70 000 tensors, one pair shared
+    n = 70000
+    many = _arrays([0x100000 + 64 * ((i * 7919) % n) for i in range(n)], [16] * n, [1] * n)
+    many[1][n - 1] = many[1][0]
+    assert clip(many, b=L.mbrl_optim_workspace_bytes(n)) == -7 and b"share memory" in L.mbrl_last_error()
     # gradients are only read: two parameters may have the same one, and the norm may count a tensor twice
     assert L.mbrl_grad_norm(*good, 5, ws, big, norm, None) == -7
 
