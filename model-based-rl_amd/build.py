@@ -32,6 +32,10 @@ def needs_build():
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+# No packed float32 instructions: some of their forms have been seen to give wrong results.  (The host pass of hipcc warns that
+# it does not know the feature.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # -pragma-unroll-threshold: the tree-sparse factorisation must unroll completely (register arrays);
 # -disable-machine-licm: loop-invariant integer bookkeeping must not be hoisted into 100+ registers;
 # no-NaN / no-infinity / no-signed-zero arithmetic: lets x * 0.0 and x + 0.0 fold (model tables are full of zeros)
@@ -42,13 +46,12 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-pass
                "-mllvm", "-amdgpu-use-amdgpu-trackers=1",   # GCN register-pressure trackers in the scheduler: ~30 % fewer AGPR copies
                "-mllvm", "-amdgpu-sched-strategy=max-ilp",  # occupancy is pinned at one wave per SIMD anyway: schedule for
                                                             # latency, not for registers (-2.7 %; iterative-ilp, minreg slower)
-               "-fno-honor-nans", "-fno-honor-infinities", "-fno-signed-zeros"]
+               "-fno-honor-nans", "-fno-honor-infinities", "-fno-signed-zeros"] + NO_PACKED_FP32
 
 
 # The optimiser-step operators are a translation unit of their own: they promise IEEE results for infinities and NaN, which
-# the flags above give away, and gain nothing from that schedule.  No packed float32 instructions: some of their forms
-# have been seen to give wrong results.
-OPTIM_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# the flags above give away, and gain nothing from that schedule.
+OPTIM_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_FP32
 
 
 def compile_lib(out, extra_flags=()):
