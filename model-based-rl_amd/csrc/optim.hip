@@ -7,12 +7,23 @@
 //   Adam   g <- c g (+ wd x)          m <- b1 m + (1 - b1) g      v <- b2 v + (1 - b2) g^2
 //          x <- x (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v / (1 - b2^t)) + eps)
 //
-// Layout.  Every tensor is cut into units of 2^shift values, a unit belongs to one wave, and the units of the whole list
-// are dealt out to the waves of a launch in turn.  The list travels in the kernel arguments (at most 4 KB), so a call
-// uploads nothing, can be captured into a graph, and keeps nothing of one call for the next; a longer list takes several
-// launches.  A wave finds its unit's tensor by comparing 64 unit ends at once (owner()).  Sums are float64 in every
-// case: squares of float32 and bfloat16 values cannot overflow there, and each partial sum has a fixed place and is
-// added in a fixed order, so the norm does not depend on which wave is done first (no atomics).
+// Layout.  Every tensor is cut into units of 2^shift values, a unit belongs to one wave, and the units of the whole list are
+// spread over the waves of a launch.  The list travels in the kernel arguments (at most 4 KB), so a call uploads nothing,
+// can be captured into a graph, and keeps nothing of one call for the next; a longer list takes several launches.  A wave
+// finds its unit's tensor by comparing 64 unit ends at once (owner()).  Sums are float64 in every case: squares of float32
+// and bfloat16 values cannot overflow there, and each partial sum has a fixed place and is added in a fixed order, so the
+// norm does not depend on which wave is done first (no atomics).
+//
+// What bounds it.  Memory, from some 10 MB on: a multiplication or two a value for the norm and clipping, some 60
+// instructions (a division and a root among them) for the update.  Measured on an MI355X, where a copy of 4 GiB runs at 4.8
+// TB/s and x *= c at 5.9, float32 values, kernel arguments and all launches included:
+//   values            norm                 clip (scaled)          Adam                  Adam, clipped
+//   8e3               3.7 us               5.5 us                 6.2 us                8.4 us           one launch
+//   5e5               4.8 us               6.8 us                 6.2 us                8.3 us           two launches
+//   8e6               6.5 us, 5.0 TB/s     13.6 us, 7.0 TB/s      41 us, 5.5 TB/s       48 us            from the cache
+//   268e6             161 us, 6.6 TB/s     517 us, 6.2 TB/s       1.23 ms, 6.1 TB/s     1.39 ms          from memory
+// (clip: two reads and a write).  Below that it is the launches: an empty one takes 2.2 us of the device and 3.7 us of the
+// host, so small lists are done in one.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,14 +41,33 @@ namespace {
 using mbrl::report;
 
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kMaxBlocks = 1024;          // of a launch: 4 blocks of 4 waves a CU
+
+// Bytes that one block of 16 waves takes on alone, in one launch (of gradients; of all four tensors for Adam).  Against the two
+// launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.9 / 5.3 for 4.6 / 8.1, clipping of
+// 24e3 6.9 / 7.1 for 6.0 / 8.7, Adam of 12e3 7.2 / 7.5 for 5.5 / 9.0.  Twice as much is slower both ways for the last two.
+constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
-constexpr int kUnits = 2;                 // units of a wave, at least, where waves stay
-constexpr int kMinShift = 9, kMaxShift = 12, kSmallShift = 8;
-constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;      // bytes that one block takes on alone
-constexpr int kMaxParts = 2048;           // partial sums that every block of a second launch joins for itself
-constexpr int64_t kCache = int64_t(256) << 20;                   // bytes of the last-level cache
-constexpr int kStreamBlocks = 1 << 22;    // of a launch that does not stay: HIP counts threads in 32 bits
+constexpr int kSmallShift = 8;            // units of one 1 KB load a wave: 800-value tensors 6.6 us for 7.2 with twice that (Adam)
+
+// Middle lists: up to kMaxBlocks blocks (4 a CU) stay and take units of 2^9 values or more.  Clipping and norm walk a wave's units
+// one after another (walk()): 8e6 values 7.0 us for 10.2 dealt out in turn, 16e6 13.4 for 15.4.  Two units a wave at least:
+// 2e6 values 5.5 us for 5.9 with one.
+constexpr int kMaxBlocks = 1024, kUnits = 2;
+constexpr int kMinShift = 9, kMaxShift = 12;
+constexpr int kMaxParts = 2048;           // partial sums that every block of a second launch joins for itself, not a launch between
+
+// Large lists: what does not stay in the 256 MB last-level cache is read and written past it (nontemporal), and the scaling and
+// the update take short units in blocks that do not stay, so that what is under way at a time lies together.  268e6 float32
+// values: norm 161 us for 180, scaling 357 for 440, Adam 1226 for 1505.  From a quarter of the cache on it pays for data that
+// was not in it (float32, other tensors used between: clipping of 32e6 values 67 us for 81, Adam of 8e6 43 for 51; of 4e6 26
+// for 28) and costs little for data that was (65 -> 71, 38 -> 41).  A norm alone gains from half of it on (32e6: 25.2 us for
+// 27.1; 16e6: 17.3 for 17.0); before a scaling it leaves what it reads in the cache, up to its size (64e6: 126 us for 131).
+constexpr int64_t kCache = int64_t(256) << 20;
+// Values of a unit: of the update one 16-byte load a lane and tensor (268e6 values: 1216 us for 1321 with two), of the scaling
+// four (496 us for 548 with two, 514 with eight).  Two units a wave of the scaling, for lists that need none: its blocks alone
+// take 11 us for 22 with one.
+constexpr int kAdamShift = 8, kScaleShift = 10, kScaleShift16 = 11;
+constexpr int kStreamBlocks = 1 << 22;    // HIP counts a launch's threads in 32 bits
 
 // ---- element types: what is stored, what is computed with, values in 16 bytes ----
 struct F64 { using T = double; using C = double; static constexpr int V = 2; };
@@ -48,7 +78,7 @@ struct F16 { using T = _Float16; using C = float; static constexpr int V = 8; };
 // Vectors with the alignment of their elements: a tensor may start at any element (a slice of a bucket), and the memory
 // system takes a 16-byte access at any such address, so there is one path for all alignments.
 template <class T, int V> struct Pack { T v[V]; };
-template <int kBytes, int kAlign> struct Raw { typedef uint32_t type __attribute__((ext_vector_type(kBytes / 4), aligned(kAlign))); };
+template <int kBytes, int kAlign> struct Raw { typedef uint32_t type __attribute__((ext_vector_type(kBytes / 4), aligned(kAlign), may_alias)); };
 template <bool kStream, int V, class T>
 __device__ __forceinline__ Pack<T, V> load(const T *p) {
     using R = typename Raw<int(sizeof(Pack<T, V>)), int(sizeof(T))>::type;
@@ -63,7 +93,7 @@ __device__ __forceinline__ void store(T *p, const Pack<T, V> &r) {
     else *q = __builtin_bit_cast(R, r);
 }
 
-// Calls f(integral_constant-like element type) for a stored type code; wave-uniform.
+// Calls f(the element type) for a type code, which is the same in all lanes.
 template <class F>
 __device__ __forceinline__ void by_type(int code, F &&f) {
     if (code == MBRL_DT_FLOAT) f(F32{});
@@ -85,6 +115,7 @@ template <int K> struct BeginList { Units<K> u; const void *x[K]; float *step[K]
 template <int K> struct UpdateList { Units<K> u; const void *x[K]; void *p[K], *m[K], *v[K]; };
 template <int K> struct SmallList { UpdateList<K> l; float *step[K]; double lr[K], wd[K]; };                    // both, for one launch
 template <int K> struct CountList { float *step[K]; double lr[K], wd[K]; int count; };
+// How many fit 4 KB, and a size of its own for few: filling 4 KB of arguments takes the host 0.5 us more than 350 bytes.
 constexpr int kFew = 16, kNormList = 192, kAdamList = 80, kSmallList = 52, kCountList = 160;
 static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kAdamList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
               sizeof(SmallList<kSmallList>) <= 3968 && sizeof(CountList<kCountList>) <= 3968, "kernel arguments are 4 KB");
@@ -238,7 +269,13 @@ template <int P>
 __device__ __forceinline__ double join_partials(const double *part, int parts) {
     if (parts == 1) return part[0];
     double acc = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kThreads) acc = join<P>(acc, part[i]);
+    for (int i = threadIdx.x; i < parts; i += 4 * kThreads) {        // four on their way at once: other dies wrote them, it is far
+        double x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = i + k * kThreads < parts ? part[i + k * kThreads] : 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc = join<P>(acc, x[k]);
+    }
     return block_join<P, kWaves>(acc);
 }
 
@@ -294,7 +331,8 @@ __device__ __forceinline__ void piece_scale(E, void *base, const Piece &p, doubl
     if (tail < n) x[tail] = T(f(x[tail]));
 }
 
-// x * 1 is x: a factor of 1 leaves nothing to read or write.
+// Every block of a middle list joins the partial sums for itself: 0.5 us instead of a launch between.  x * 1 is x: a factor of
+// 1 leaves nothing to read or write.
 template <int P, bool kStream, class L>
 __global__ __launch_bounds__(kThreads) void clip_scale(const L l, const double *part, int parts, double max_norm, double *norm) {
     const double s = root_of<P>(join_partials<P>(part, parts)), c = factor_of(s, max_norm);
@@ -442,8 +480,7 @@ __global__ __launch_bounds__(kSmallThreads) void adam_small(const L a, const Bet
 // ---- host ----
 const int kSize[4] = {8, 4, 2, 2};
 
-// How a list's values are cut and walked.  Small: one block.  Else up to kMaxBlocks blocks stay and take unit after unit,
-// with units small enough to fill them and large enough that finding a unit's tensor does not count.
+// Units small enough to fill the blocks that stay, and large enough that finding a unit's tensor does not count.
 int unit_shift(int64_t values) {
     int shift = kMinShift;
     while (shift < kMaxShift && (values >> shift) > 4 * kMaxBlocks * kWaves) shift++;
@@ -556,7 +593,8 @@ struct Space {
 };
 
 // The gradients of a call, for a norm or scaling, to which it is all one where a tensor ends: neighbours in memory of one type
-// become one.  A bucket of many tensors is one long run then, which takes one launch instead of one for each kNormList.
+// become one.  A bucket of many tensors is one long run then, which takes one launch instead of one for each kNormList (402
+// tensors, 53 MB, clipped: 29 us for 50).
 struct Gradients {
     int64_t count, values, bytes;
     void *const *x;
@@ -596,17 +634,41 @@ struct Gradients {
     }
 };
 
-// -> how many partial sums there are
-template <int P, bool kStream, class L>
-int launch_partials(L &l, const Gradients &g, double *part, hipStream_t st) {
+// Calls f(the flag as a constant).
+template <class F> void by_flag(bool flag, F &&f) { flag ? f(std::true_type{}) : f(std::false_type{}); }
+// Calls f(a list of the smallest size): few tensors have one of their own, but where memory is what counts.
+template <template <int> class List, int K, class F>
+void by_count(int64_t count, bool stream, F &&f) {
+    if (count <= kFew && !stream) f(List<kFew>{});
+    else f(List<K>{});
+}
+
+// Joins the partial sums in a launch of its own where `finish` says so, they are too many for every block of the next launch, or
+// there are none (all tensors are empty: the next launch may have no block that would write the norm).
+struct Parts { const double *part; int parts; };
+template <int P>
+Parts launch_finish(int parts, bool finish, const Space &ws, double *norm, hipStream_t st) {
+    if (!finish && parts && parts <= kMaxParts) return {ws.part, parts};
+    hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
+    return {ws.total, 1};
+}
+
+// Launches the partial sums of a list.
+template <int P>
+Parts launch_partials(const Gradients &g, bool stream, bool finish, const Space &ws, double *norm, hipStream_t st) {
     int parts = 0;
-    g.lists(l, unit_shift(g.values), [&] {
-        if (const int grid = grid_of(l.u, kMaxBlocks, kStream ? 1 : kUnits)) {
-            hipLaunchKernelGGL((norm_partials<P, kStream, L>), dim3(grid), dim3(kThreads), 0, st, l, part + parts);
-            parts += grid;
-        }
+    by_flag(stream, [&](auto stream_) {
+        constexpr bool kStream = stream_;
+        by_count<NormList, kNormList>(g.count, kStream, [&](auto l) {
+            g.lists(l, unit_shift(g.values), [&] {
+                if (const int grid = grid_of(l.u, kMaxBlocks, kStream ? 1 : kUnits)) {
+                    hipLaunchKernelGGL((norm_partials<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
+                    parts += grid;
+                }
+            });
+        });
     });
-    return parts;
+    return launch_finish<P>(parts, finish, ws, norm, st);
 }
 
 // The norm of a list, and the scaling where kClip.
@@ -615,34 +677,26 @@ void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm,
     by_norm(kind, [&](auto P_) {
         constexpr int P = P_;
         if constexpr (P != kNoClip) {
-            auto small = [&](auto l) {
-                g.lists(l, kSmallShift, [] {});
-                hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
-            };
-            auto large = [&](auto l, auto stream) {
-                constexpr bool kStream = stream;
-                int parts = launch_partials<P, kStream>(l, g, ws.part, st);
-                const double *part = ws.part;
-                if (!kClip || kStream || parts > kMaxParts || !parts) {        // !parts: all tensors empty, no block below that would write the norm
-                    hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
-                    part = ws.total;
-                    parts = 1;
-                }
-                if constexpr (kClip)
-                    g.lists(l, kStream ? (g.bytes == 2 * g.values ? 11 : 10) : unit_shift(g.values), [&] {
-                        if (const int grid = kStream ? grid_of(l.u, kStreamBlocks) : grid_of(l.u, kMaxBlocks, kUnits))
-                            hipLaunchKernelGGL((clip_scale<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, part, parts, max_norm, norm);
-                    });
-            };
             if (g.bytes <= (kClip ? kSmallClip : kSmallNorm) && g.count <= kNormList) {
-                if (g.count <= kFew) small(NormList<kFew>{});
-                else small(NormList<kNormList>{});
-            } else if (g.bytes > kCache) {
-                large(NormList<kNormList>{}, std::true_type{});
-            } else {
-                if (g.count <= kFew) large(NormList<kFew>{}, std::false_type{});
-                else large(NormList<kNormList>{}, std::false_type{});
+                by_count<NormList, kNormList>(g.count, false, [&](auto l) {
+                    g.lists(l, kSmallShift, [] {});
+                    hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
+                });
+                return;
             }
+            const bool stream = g.bytes > kCache / 4;
+            const Parts sum = launch_partials<P>(g, g.bytes > (kClip ? kCache : kCache / 2), !kClip || stream, ws, norm, st);
+            if constexpr (kClip)
+                by_flag(stream, [&](auto stream_) {
+                    constexpr bool kStream = stream_;
+                    by_count<NormList, kNormList>(g.count, kStream, [&](auto l) {
+                        g.lists(l, !kStream ? unit_shift(g.values) : g.bytes == 2 * g.values ? kScaleShift16 : kScaleShift, [&] {
+                            if (const int grid = grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks, kUnits))
+                                hipLaunchKernelGGL((clip_scale<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, sum.part, sum.parts,
+                                                   max_norm, norm);
+                        });
+                    });
+                });
         }
     });
 }
@@ -749,60 +803,51 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         auto counters = [&](auto &l) { return [&](int at, int64_t k) { l.step[at] = steps[k]; l.lr[at] = lr[k]; l.wd[at] = weight_decay[k]; }; };
         by_norm(clip ? norm_type : kNoClip, [&](auto P_) {
             constexpr int P = P_;
-            auto small = [&](auto l) {
-                lists(l.l, kSmallShift, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
-                hipLaunchKernelGGL((adam_small<P, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, b, decoupled, max_norm, norm);
-            };
-            auto large = [&](auto begin, auto update, auto stream) {
-                constexpr bool kStream = stream;
-                const int shift = unit_shift(values);
-                int parts = 0;
-                if (count <= kAdamList) {
-                    lists(begin, shift, counters(begin), [&](int64_t) {
-                        parts = clip ? std::max(grid_of(begin.u), 1) : 1;
-                        hipLaunchKernelGGL((adam_begin<P, kStream, decltype(begin)>), dim3(parts), dim3(kThreads), 0, st, begin, b, decoupled,
-                                           ws.scalars, ws.part);
-                    });
-                } else {
-                    CountList<kCountList> l;
-                    for (int64_t i = 0; i < count; i += kCountList) {
-                        l.count = int(std::min<int64_t>(count - i, kCountList));
-                        for (int k = 0; k < l.count; k++) counters(l)(k, i + k);
-                        hipLaunchKernelGGL(adam_count, dim3(1), dim3(kCountList), 0, st, l, b, decoupled, ws.scalars + i);
-                    }
-                    if constexpr (P != kNoClip) {
-                        const Gradients g(count, const_cast<void *const *>(grads), numel, dtype);
-                        if (g.count <= kFew && !kStream) {
-                            NormList<kFew> few;
-                            parts = launch_partials<P, false>(few, g, ws.part, st);
-                        } else {
-                            NormList<kNormList> many;
-                            parts = launch_partials<P, kStream>(many, g, ws.part, st);
-                        }
-                    }
-                }
-                const double *part = ws.part;
-                if constexpr (P != kNoClip)
-                    if (kStream || parts > kMaxParts) {
-                        hipLaunchKernelGGL((norm_finish<P>), dim3(1), dim3(kThreads), 0, st, ws.part, parts, ws.total, norm);
-                        part = ws.total;
-                        parts = 1;
-                    }
-                lists(update, kStream ? 8 : shift, tensors(update), [&](int64_t i) {
-                    if (const int grid = std::max(grid_of(update.u, kStream ? kStreamBlocks : kMaxBlocks), clip && i == 0 ? 1 : 0))        // one block at least writes the norm
-                        hipLaunchKernelGGL((adam_update<P, kStream, decltype(update)>), dim3(grid), dim3(kThreads), 0, st, update, b,
-                                           ws.scalars + i, part, parts, max_norm, norm);
-                });
-            };
+            constexpr bool kClip = P != kNoClip;
             if (bytes <= kSmallAdam && count <= kSmallList) {
-                if (count <= kFew) small(SmallList<kFew>{});
-                else small(SmallList<kSmallList>{});
-            } else if (bytes > kCache) {
-                large(BeginList<kAdamList>{}, UpdateList<kAdamList>{}, std::true_type{});
-            } else {
-                if (count <= kFew) large(BeginList<kFew>{}, UpdateList<kFew>{}, std::false_type{});
-                else large(BeginList<kAdamList>{}, UpdateList<kAdamList>{}, std::false_type{});
+                by_count<SmallList, kSmallList>(count, false, [&](auto l) {
+                    lists(l.l, kSmallShift, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
+                    hipLaunchKernelGGL((adam_small<P, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, b, decoupled, max_norm, norm);
+                });
+                return;
             }
+            const bool stream = bytes > kCache / 4;
+            const int shift = unit_shift(values);
+            Parts sum{nullptr, 0};
+            if (count <= kAdamList) {
+                by_flag(kClip && total_bytes(count, numel, dtype) > kCache, [&](auto stream_) {
+                    constexpr bool kStream = kClip && stream_;
+                    by_count<BeginList, kAdamList>(count, kStream, [&](auto l) {
+                        lists(l, shift, counters(l), [&](int64_t) {
+                            const int grid = kClip ? std::max(grid_of(l.u), 1) : 1;
+                            hipLaunchKernelGGL((adam_begin<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, decoupled,
+                                               ws.scalars, ws.part);
+                            if constexpr (kClip) sum = launch_finish<P>(grid, stream, ws, norm, st);
+                        });
+                    });
+                });
+            } else {
+                CountList<kCountList> l;
+                for (int64_t i = 0; i < count; i += kCountList) {
+                    l.count = int(std::min<int64_t>(count - i, kCountList));
+                    for (int k = 0; k < l.count; k++) counters(l)(k, i + k);
+                    hipLaunchKernelGGL(adam_count, dim3(1), dim3(kCountList), 0, st, l, b, decoupled, ws.scalars + i);
+                }
+                if constexpr (kClip) {
+                    const Gradients g(count, const_cast<void *const *>(grads), numel, dtype);
+                    sum = launch_partials<P>(g, g.bytes > kCache, stream, ws, norm, st);
+                }
+            }
+            by_flag(stream, [&](auto stream_) {
+                constexpr bool kStream = stream_;
+                by_count<UpdateList, kAdamList>(count, kStream, [&](auto l) {
+                    lists(l, kStream ? kAdamShift : shift, tensors(l), [&](int64_t i) {
+                        if (const int grid = std::max(grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks), kClip && i == 0 ? 1 : 0))        // one block at least writes the norm
+                            hipLaunchKernelGGL((adam_update<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, ws.scalars + i,
+                                               sum.part, sum.parts, max_norm, norm);
+                    });
+                });
+            });
         });
         return launched("mbrl_adam_step");
     });

@@ -100,8 +100,6 @@ class FusedAdam(torch.optim.Optimizer):
     def _common(self):
         first = self.param_groups[0]
         for g in self.param_groups:
-            if g.get("amsgrad") or g.get("maximize"):
-                raise ValueError("FusedAdam: amsgrad and maximize are not offered")
             for k in ("betas", "eps", "decoupled_weight_decay"):
                 if g[k] is not first[k] and g[k] != first[k]:
                     raise ValueError("FusedAdam: %s has to be the same in all parameter groups" % k)
@@ -127,7 +125,9 @@ class FusedAdam(torch.optim.Optimizer):
                 g = p.grad
                 if g is None:
                     continue
-                s = state.get(p) or self._new_state(p)
+                s = state[p]
+                if "exp_avg" not in s:
+                    self._new_state(p)
                 params.append(p)
                 grads.append(g)
                 avgs.append(s["exp_avg"])
@@ -140,20 +140,23 @@ class FusedAdam(torch.optim.Optimizer):
                                        first["decoupled_weight_decay"], self.max_norm, self.norm_type)
         return loss
 
+    def __getstate__(self):        # for copies and pickles; the base class keeps its own three attributes only
+        return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type, grad_norm=None)
+
     def load_state_dict(self, state_dict):
         """As Optimizer.load_state_dict, but moments keep their float32 (or float64) values: the base class rounds them to
         their parameter's type."""
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]) or \
+                any("max_exp_avg_sq" in s for s in state_dict["state"].values()):
+            raise ValueError("FusedAdam: amsgrad and maximize are not offered")
         super().load_state_dict(state_dict)
         for g in self.param_groups:
             g.setdefault("decoupled_weight_decay", self.defaults["decoupled_weight_decay"])
-        self._common()
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             saved = state_dict["state"].get(i)
-            if not saved:
+            if not saved or "exp_avg" not in saved:
                 continue
-            if "max_exp_avg_sq" in saved:
-                raise ValueError("FusedAdam: amsgrad and maximize are not offered")
             s = self._new_state(p)
             s["step"].copy_(torch.as_tensor(saved["step"], dtype=torch.float32))
             for k in ("exp_avg", "exp_avg_sq"):

@@ -126,6 +126,8 @@ def do_training(cfg, logger, output_results_dir, output_rec_dir, output_weights_
         output["average_sd"].append(float(np.mean(policy.get_clamped_sd())))
         if rank == 0 and epoch_idx % cfg.LOG.PERIOD == 0:
             logger.info("REWARD: \t\t{} (iteration {})".format(loss["objective_loss"], epoch_idx))
+            if "grad_norm" in loss:          # SOLVER.CLIP_GRAD_NORM
+                logger.info("GRADIENT NORM: \t{} (iteration {})".format(loss["grad_norm"], epoch_idx))
         if rank == 0 and epoch_idx % cfg.LOG.CHECKPOINT_PERIOD == 0:
             torch.save(model.state_dict(), os.path.join(output_weights_dir, "iter_{}.pth".format(epoch_idx)))
 

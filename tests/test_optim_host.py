@@ -1,5 +1,6 @@
 """CPU: what the optimiser-step operators (optim.py, include/mbrl.h) refuse -- all of it is decided on the host, before any
 launch -- and how the strategy and its optimiser reach them."""
+import copy
 import ctypes as C
 import math
 
@@ -149,6 +150,13 @@ def test_fused_adam_construction_and_state_dict():
     assert torch.equal(again.state[p[1]]["exp_avg"], opt.state[p[1]]["exp_avg"])
     ref.load_state_dict(opt.state_dict())        # and back
     assert float(ref.state[p[0]]["step"]) == 7.0
+    twin = copy.deepcopy(optim.FusedAdam(p, 0.1, max_norm=3.0, norm_type=1))
+    assert (twin.max_norm, twin.norm_type, twin.grad_norm) == (3.0, 1, None)
+    opt.state[p[0]].clear()
+    opt.state[p[0]]["mine"] = 1                  # another's entry does not pass for the state
+    with pytest.raises(lib.MbrlError, match="no CPU path"):
+        opt.step()
+    assert float(opt.state[p[0]]["step"]) == 0.0 and opt.state[p[0]]["mine"] == 1
     with pytest.raises(ValueError, match="amsgrad"):
         opt.load_state_dict(torch.optim.Adam(p, amsgrad=True).state_dict())
 
