@@ -42,6 +42,17 @@ int type_code(at::ScalarType t) {
     }
 }
 
+struct List;
+// The GPU that all tensors of a call are on, or the first one that is not.
+struct Place {
+    c10::Device device{c10::DeviceType::CPU};
+    const List *wrong = nullptr;
+    size_t index = 0;
+    bool elsewhere = false;
+    void met(const List &l, size_t i, const at::Tensor &x);
+    void settle() const;
+};
+
 // The tensors of a list (or any iterable), as a tuple of its own: the caller's list may change while numbers are converted.
 struct List {
     PyObject *seq = nullptr;
@@ -70,24 +81,34 @@ struct List {
     [[noreturn]] void bad(size_t i, PyObject *type, const std::string &why) const {
         raise(type, std::string(name) + ": element " + std::to_string(i) + " " + why);
     }
-    void check_layout(size_t i) const {
+    // Refuses what no operator takes, and gets the address.  A tensor off the device is refused last, by settle(): what is wrong
+    // with a list is said without a GPU too.
+    void check(size_t i, Place &at) {
         const at::Tensor &x = *t[i];
         if (!x.defined() || x.layout() != at::kStrided) bad(i, PyExc_ValueError, "is not a dense (strided) tensor");
         if (x.is_neg()) bad(i, PyExc_ValueError, "is a lazily negated view (resolve_neg() it)");
         if (!x.is_non_overlapping_and_dense())
             bad(i, PyExc_ValueError, "has gaps or repeated values between its strides (use .contiguous())");
-    }
-    // Last of the checks: all tensors on one GPU.  Takes their addresses.
-    void locate(c10::Device &dev) {
-        for (size_t i = 0; i < t.size(); i++) {
-            const at::Tensor &x = *t[i];
-            if (!x.is_cuda()) bad(i, mbrl_error, "is not on a GPU (these operators run only on the HIP device; there is no CPU path)");
-            if (dev.type() != c10::DeviceType::CUDA) dev = x.device();
-            else if (x.device() != dev) bad(i, PyExc_ValueError, "is on another GPU than the first tensor (one process per GPU)");
-            ptr[i] = x.numel() ? x.data_ptr() : nullptr;
-        }
+        if (at.device != x.device() || !x.is_cuda()) at.met(*this, i, x);
+        ptr[i] = x.numel() ? x.data_ptr() : nullptr;
     }
 };
+
+inline void Place::met(const List &l, size_t i, const at::Tensor &x) {
+    if (wrong) return;
+    if (x.is_cuda() && device.type() != c10::DeviceType::CUDA) {
+        device = x.device();
+        return;
+    }
+    wrong = &l;
+    index = i;
+    elsewhere = x.is_cuda();
+}
+inline void Place::settle() const {
+    if (!wrong) return;
+    if (elsewhere) wrong->bad(index, PyExc_ValueError, "is on another GPU than the first tensor (one process per GPU)");
+    wrong->bad(index, mbrl_error, "is not on a GPU (these operators run only on the HIP device; there is no CPU path)");
+}
 
 void written(const at::Tensor &x) {        // in-place changes count, for autograd and for whoever watches _version
     if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
@@ -232,13 +253,13 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         List g(a[0], "grads");
         const int kind = norm_code(a[1]);
         Sizes s(g.t.size());
+        Place at;
         for (size_t i = 0; i < g.t.size(); i++) {
-            g.check_layout(i);
+            g.check(i, at);
             type_of(g, i, s);
         }
-        c10::Device dev(c10::DeviceType::CPU);
-        g.locate(dev);
-        Call c(dev, g.t.size(), true);
+        at.settle();
+        Call c(at.device, g.t.size(), true);
         done(grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, c.space.data_ptr(), c.space.numel(), c.norm_ptr(), c.stream));
         return c.result();
     });
@@ -252,13 +273,13 @@ PyObject *py_clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const double most = limit(a[1]);
         const int kind = norm_code(a[2]);
         Sizes s(g.t.size());
+        Place at;
         for (size_t i = 0; i < g.t.size(); i++) {
-            g.check_layout(i);
+            g.check(i, at);
             type_of(g, i, s);
         }
-        c10::Device dev(c10::DeviceType::CPU);
-        g.locate(dev);
-        Call c(dev, g.t.size(), true);
+        at.settle();
+        Call c(at.device, g.t.size(), true);
         done(clip_grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, most, c.space.data_ptr(), c.space.numel(),
                             c.norm_ptr(), c.stream));
         for (const at::Tensor *x : g.t) written(*x);
@@ -282,8 +303,9 @@ PyObject *py_adam_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const double most = clip ? limit(a[11]) : 0.0;
         const int kind = norm_code(a[12]);
         Sizes s(count);
+        Place at;
         for (size_t i = 0; i < count; i++) {
-            p.check_layout(i);
+            p.check(i, at);
             type_of(p, i, s);
             const at::Tensor &x = *p.t[i];
             const at::ScalarType wide = x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
@@ -292,19 +314,18 @@ PyObject *py_adam_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
                 if (y.scalar_type() != (l == &g ? x.scalar_type() : wide))
                     l->bad(i, PyExc_ValueError, l == &g ? "has another type than its parameter" : "is not float32 (float64 for a float64 parameter)");
                 if (y.sizes() != x.sizes()) l->bad(i, PyExc_ValueError, "has another shape than its parameter");
-                l->check_layout(i);
+                l->check(i, at);
                 // the order of values in memory is what counts: strides of dimensions with one value say nothing of it
-                if (y.strides() != x.strides() && !(x.is_contiguous() && y.is_contiguous())) {
+                if (!(x.is_contiguous() && y.is_contiguous()) && y.strides() != x.strides())
                     for (int64_t d = 0; d < x.dim(); d++)
                         if (x.size(d) > 1 && x.numel() && x.stride(d) != y.stride(d))
                             l->bad(i, PyExc_ValueError, "has its values in another order than its parameter (strides differ)");
-                }
             }
             if (t.t[i]->scalar_type() != at::kFloat || t.t[i]->numel() != 1) t.bad(i, PyExc_ValueError, "is not one float32 value");
+            t.check(i, at);
         }
-        c10::Device dev(c10::DeviceType::CPU);
-        for (List *l : {&p, &g, &m, &v, &t}) l->locate(dev);
-        Call c(dev, count, clip);
+        at.settle();
+        Call c(at.device, count, clip);
         std::vector<float *> steps(count);
         for (size_t i = 0; i < count; i++) steps[i] = static_cast<float *>(t.ptr[i]);
         done(adam_step(count, p.ptr.data(), g.ptr.data(), m.ptr.data(), v.ptr.data(), steps.data(), s.numel.data(), s.dtype.data(), lr.data(),
