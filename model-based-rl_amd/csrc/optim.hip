@@ -63,10 +63,11 @@ constexpr int kMaxParts = 2048;           // partial sums that every block of a 
 // for 28) and costs little for data that was (65 -> 71, 38 -> 41).  A norm alone gains from half of it on (32e6: 25.2 us for
 // 27.1; 16e6: 17.3 for 17.0); before a scaling it leaves what it reads in the cache, up to its size (64e6: 126 us for 131).
 constexpr int64_t kCache = int64_t(256) << 20;
-// Values of a unit: of the update one 16-byte load a lane and tensor (268e6 values: 1216 us for 1321 with two), of the scaling
-// four (496 us for 548 with two, 514 with eight).  Two units a wave of the scaling, for lists that need none: its blocks alone
-// take 11 us for 22 with one.
-constexpr int kAdamShift = 8, kScaleShift = 10, kScaleShift16 = 11;
+// Values of a unit.  Of the update one load a lane and tensor (268e6 float32 values: 1.23 ms for 1.30 with two, bfloat16 0.93 for
+// 1.04; 128e6 of float64, half as many a load: 1.19 for 1.25), compiled for that alone: 72 registers for 117 leave room for 7
+// waves for 4 (bfloat16 0.93 ms for 1.08).  Of the scaling four loads (496 us for 548 with two, 514 with eight), and two units
+// a wave, for lists that need no scaling: its blocks alone take 11 us for 22 with one.
+constexpr int kAdamShift = 8, kAdamShift64 = 7, kScaleShift = 10, kScaleShift16 = 11;
 constexpr int kStreamBlocks = 1 << 22;    // HIP counts a launch's threads in 32 bits
 
 // ---- element types: what is stored, what is computed with, values in 16 bytes ----
@@ -105,7 +106,7 @@ __device__ __forceinline__ void by_type(int code, F &&f) {
 // ---- lists in kernel arguments ----
 template <int K_> struct Units {
     static constexpr int K = K_;
-    uint64_t n[K];        // values << 2 | type code
+    uint64_t n[K];        // values << 8 | head << 2 | type code
     uint32_t end[K];      // units of the tensors up to and including this one
     int count, shift;
     uint32_t units;
@@ -127,29 +128,35 @@ __device__ __forceinline__ uint32_t wave_of_block() { return __builtin_amdgcn_re
 __device__ __forceinline__ uint32_t wave_of_grid() { return blockIdx.x * kWaves + wave_of_block(); }
 __device__ __forceinline__ uint32_t waves_of_grid() { return gridDim.x * kWaves; }
 
-// The tensor that unit `unit` belongs to: as many as end at or before it come first.
+// The tensor that unit `unit` belongs to: as many as end at or before it come first.  All ends are on their way at once.
 template <class U>
 __device__ __forceinline__ int owner(const U &u, uint32_t unit) {
     const int lane = threadIdx.x % kWave;
+    uint32_t end[(U::K + kWave - 1) / kWave];
+#pragma unroll
+    for (int k = 0; k < U::K; k += kWave) end[k / kWave] = u.end[min(k + lane, u.count - 1)];
     int t = 0;
-    for (int k = 0; k < u.count; k += kWave)
-        t += __popcll(__ballot(k + lane < u.count && u.end[k + lane < u.count ? k + lane : 0] <= unit));
+#pragma unroll
+    for (int k = 0; k < U::K; k += kWave) t += __popcll(__ballot(k + lane < u.count && end[k / kWave] <= unit));
     return __builtin_amdgcn_readfirstlane(t);
 }
 
-// Values of one tensor, one after another.
-struct Piece { int t, type; int64_t first; int n; };
+// Values of one tensor, one after another: n from `first` on, which begins a cache line, and where the tensor begins the `head`
+// before the first line.
+struct Piece { int t, type, head; int64_t first; int n; };
 
-// Units `unit` to `stop` of the list, as far as they lie in one tensor; moves `unit` past them.
+// Units `unit` to `stop` of the list, as far as they lie in tensor t; moves `unit` past them.
 template <class U>
-__device__ __forceinline__ Piece piece(const U &u, uint32_t &unit, uint32_t stop) {
+__device__ __forceinline__ Piece piece(const U &u, int t, uint32_t &unit, uint32_t stop) {
     Piece p;
-    p.t = owner(u, unit);
-    const uint64_t n = u.n[p.t];
-    const uint32_t end = min(stop, u.end[p.t]), skipped = unit - (p.t ? u.end[p.t - 1] : 0);
+    p.t = t;
+    const uint64_t n = u.n[t];
+    const uint32_t end = min(stop, u.end[t]), skipped = unit - (t ? u.end[t - 1] : 0);
+    const int head = int(n >> 2 & 63);
     p.type = int(n & 3);
-    p.first = int64_t(skipped) << u.shift;
-    p.n = int(min(int64_t(n >> 2) - p.first, int64_t(end - unit) << u.shift));
+    p.head = skipped ? 0 : head;
+    p.first = head + (int64_t(skipped) << u.shift);
+    p.n = int(min(int64_t(n >> 8) - p.first, int64_t(end - unit) << u.shift));
     unit = end;
     return p;
 }
@@ -159,14 +166,17 @@ template <class U, class F>
 __device__ __forceinline__ void dealt(const U &u, uint32_t wave, uint32_t waves, F f) {
     for (uint32_t i = wave; i < u.units; i += waves) {
         uint32_t unit = i;
-        f(piece(u, unit, unit + 1));
+        f(piece(u, owner(u, unit), unit, unit + 1));
     }
 }
 // The same, but units one after another, so that a wave has few tensors to find.
 template <class U, class F>
 __device__ __forceinline__ void shared_out(const U &u, uint32_t wave, uint32_t waves, F f) {
     const uint32_t each = (u.units + waves - 1) / waves, stop = min(u.units, (wave + 1) * each);
-    for (uint32_t unit = wave * each; unit < stop;) f(piece(u, unit, stop));
+    uint32_t unit = wave * each;
+    if (unit >= stop) return;
+    for (int t = owner(u, unit); unit < stop; t++)
+        if (u.end[t] > unit) f(piece(u, t, unit, stop));        // an empty tensor ends where it begins
 }
 template <bool kStream, class U, class F>
 __device__ __forceinline__ void walk(const U &u, F f) {
@@ -227,8 +237,9 @@ __device__ __forceinline__ double piece_norm(E, const void *base, const Piece &p
 #pragma unroll
         for (int j = 0; j < V; j++) a[j % 2] = add<P>(a[j % 2], double(typename E::C(r.v[j])));
     }
-    const int tail = n / V * V + lane;        // the last n % V values, one a lane
+    const int tail = n / V * V + lane;        // the last n % V values, one a lane, and those of the head
     if (tail < n) a[1] = add<P>(a[1], double(typename E::C(x[tail])));
+    if (lane < p.head) a[1] = add<P>(a[1], double(typename E::C(static_cast<const T *>(base)[lane])));
     return join<P>(a[0], a[1]);
 }
 
@@ -329,6 +340,7 @@ __device__ __forceinline__ void piece_scale(E, void *base, const Piece &p, doubl
     }
     const int tail = n / V * V + lane;
     if (tail < n) x[tail] = T(f(x[tail]));
+    if (lane < p.head) x[lane - p.first] = T(f(x[lane - p.first]));
 }
 
 // Every block of a middle list joins the partial sums for itself: 0.5 us instead of a launch between.  x * 1 is x: a factor of
@@ -419,10 +431,13 @@ __device__ __forceinline__ void piece_adam(E, const L &l, const Piece &q, const 
         }
     };
     int i = lane * V;
-    for (; i + kStep + V <= n; i += 2 * kStep) some(i, std::integral_constant<int, 2>{});
-    if (i + V <= n) some(i, std::integral_constant<int, 1>{});
+    if constexpr (!kStream)        // where units have one vector a lane, two at once would only take registers, and with them waves
+        for (; i + kStep + V <= n; i += 2 * kStep) some(i, std::integral_constant<int, 2>{});
+    for (; i + V <= n; i += kStep) some(i, std::integral_constant<int, 1>{});
+    auto one = [&](int64_t i) { p[i] = T(f(C(p[i]), C(g[i]), m[i], v[i])); };
     const int tail = n / V * V + lane;
-    if (tail < n) p[tail] = T(f(C(p[tail]), C(g[tail]), m[tail], v[tail]));
+    if (tail < n) one(tail);
+    if (lane < q.head) one(lane - q.first);
 }
 
 constexpr int kNoClip = -1;        // P of an update that does not clip
@@ -499,14 +514,18 @@ int64_t total_bytes(int64_t count, const int64_t *numel, const int *dtype) {
     return n;
 }
 
-// Puts tensors `from` to `to` of a call into a list: fill(list, place, tensor).  Empty ones have a place and no units.
-template <class List, class Fill>
-void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const int *dtype, int shift, Fill fill) {
+// Puts tensors `from` to `to` of a call into a list: fill(place, tensor).  Empty ones have a place and no units.  Units begin at
+// cache lines of the tensor at `anchor` (of values of `size(i)` bytes): 402 tensors of a bucket, which begin anywhere, are
+// updated in 261 us for 281 us from their first values on.
+constexpr int kLine = 128;
+template <class List, class Anchor, class Size, class Fill>
+void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const int *dtype, int shift, Anchor anchor, Size size, Fill fill) {
     uint32_t units = 0;
     for (int64_t i = from; i < to; i++) {
         const int at = int(i - from);
-        units += uint32_t((numel[i] + (int64_t(1) << shift) - 1) >> shift);
-        l.u.n[at] = uint64_t(numel[i]) << 2 | uint64_t(dtype[i]);
+        const int64_t head = std::min<int64_t>(numel[i], (-uintptr_t(anchor[i]) & (kLine - 1)) / size(i));
+        if (numel[i]) units += uint32_t(std::max<int64_t>((numel[i] - head + (int64_t(1) << shift) - 1) >> shift, 1));
+        l.u.n[at] = uint64_t(numel[i]) << 8 | uint64_t(head) << 2 | uint64_t(dtype[i]);
         l.u.end[at] = units;
         fill(at, i);
     }
@@ -526,7 +545,7 @@ void by_norm(int kind, F &&f) {
     else f(std::integral_constant<int, kNoClip>{});
 }
 
-constexpr int64_t kMaxValues = int64_t(1) << 38;        // of a call: units are counted in 32 bits
+constexpr int64_t kMaxValues = int64_t(1) << 37;        // of a call: units are counted in 32 bits
 
 int check_list(const char *what, int64_t count, const int64_t *numel, const int *dtype) {
     static thread_local char text[160];
@@ -628,7 +647,8 @@ struct Gradients {
         constexpr int K = decltype(l.u)::K;
         l.u.count = l.u.units = 0;
         for (int64_t i = 0; i < count; i += K) {
-            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = x[k]; });
+            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, x, [&](int64_t k) { return kSize[dtype[k]]; },
+                      [&](int at, int64_t k) { l.x[at] = x[k]; });
             go();
         }
     }
@@ -795,7 +815,8 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             constexpr int K = std::decay_t<decltype(l.u)>::K;
             l.u.count = l.u.units = 0;
             for (int64_t i = 0; i < count; i += K) {
-                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, [&](int at, int64_t k) { l.x[at] = grads[k]; fill(at, k); });
+                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, exp_avgs, [&](int64_t k) { return kSize[dtype[k]] == 8 ? 8 : 4; },
+                          [&](int at, int64_t k) { l.x[at] = grads[k]; fill(at, k); });
                 go(i);
             }
         };
@@ -841,7 +862,7 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             by_flag(stream, [&](auto stream_) {
                 constexpr bool kStream = stream_;
                 by_count<UpdateList, kAdamList>(count, kStream, [&](auto l) {
-                    lists(l, kStream ? kAdamShift : shift, tensors(l), [&](int64_t i) {
+                    lists(l, !kStream ? shift : bytes == 32 * values ? kAdamShift64 : kAdamShift, tensors(l), [&](int64_t i) {
                         if (const int grid = std::max(grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks), kClip && i == 0 ? 1 : 0))        // one block at least writes the norm
                             hipLaunchKernelGGL((adam_update<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, ws.scalars + i,
                                                sum.part, sum.parts, max_norm, norm);
