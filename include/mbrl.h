@@ -212,10 +212,12 @@ int mbrl_lane_map(int nq, int nv, int nu, int fd_mode, int *units_per_pair, int 
  * element types (MBRL_DT_*; lists may mix them).  Each tensor is a dense run of values that starts at any element; the order
  * of the values within it does not matter as long as a parameter, its gradient and its moments have the same.
  * The host arrays are read before the call returns and not kept.  `workspace`: caller-owned device memory, 256-byte
- * aligned, at least mbrl_optim_workspace_bytes(count) bytes, contents arbitrary before and after; one per call in flight
- * (calls on the same stream may share one, captured graphs that can run at the same time must not).  All launches go to the
+ * aligned, at least mbrl_optim_workspace_bytes(op, the call's list) bytes (0 for short lists: NULL will do), contents
+ * arbitrary before and after; one per call in flight (calls on the same stream may share one, captured graphs that can run
+ * at the same time must not).  All launches go to the
  * calling thread's current HIP device, which must own the memory and the stream; no call waits for the device, and all can
- * be captured into a HIP graph.  Results do not depend on timing: no atomics, every sum in a fixed order. */
+ * be captured into a HIP graph.  Results depend on the values, sizes and types alone, not on timing or addresses: no atomics,
+ * every sum in a fixed order. */
 #define MBRL_DT_DOUBLE 0
 #define MBRL_DT_FLOAT 1
 #define MBRL_DT_BFLOAT 2
@@ -223,7 +225,10 @@ int mbrl_lane_map(int nq, int nv, int nu, int fd_mode, int *units_per_pair, int 
 #define MBRL_NORM_INF 0        /* max |x| */
 #define MBRL_NORM_ONE 1        /* sum |x| */
 #define MBRL_NORM_TWO 2        /* sqrt(sum x^2) */
-int64_t mbrl_optim_workspace_bytes(int64_t count);
+#define MBRL_OP_NORM 0         /* mbrl_grad_norm */
+#define MBRL_OP_CLIP 1         /* mbrl_clip_grad_norm */
+#define MBRL_OP_ADAM 2         /* mbrl_adam_step */
+int64_t mbrl_optim_workspace_bytes(int op, int64_t count, const int64_t *numel, const int *dtype);
 
 /* norm[0] (device) = the norm over all values of all tensors, summed in fp64; 0 for an empty list; NaN if any value is.
  * Squares of fp64 values beyond 1e154 overflow to an infinite norm. */
@@ -242,7 +247,7 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
  *     param = param * (decoupled ? 1 - lr[i] weight_decay[i] : 1) - lr[i] / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps).
  * exp_avgs (m) and exp_avg_sqs (v) are fp64 for fp64 parameters and fp32 for all others; gradients have their parameter's
  * type and are left as they are.  Arithmetic in the moments' type, one rounding to a 16-bit parameter.  steps[i]: one
- * fp32 value in device memory for each tensor.  norm != NULL: the norm over all gradients is left there (device).
+ * fp32 value in device memory for each tensor, empty ones too (exact up to 2^24 steps).  norm != NULL: the norm over all gradients is left there (device).
  * Memory that is written and shared with another tensor of the call is refused (-7). */
 int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads, void *const *exp_avgs,
                    void *const *exp_avg_sqs, float *const *steps, const int64_t *numel, const int *dtype, const double *lr,

@@ -12,7 +12,7 @@
 // can be captured into a graph, and keeps nothing of one call for the next; a longer list takes several launches.  A wave
 // finds its unit's tensor by comparing 64 unit ends at once (owner()).  Sums are float64 in every case: squares of float32
 // and bfloat16 values cannot overflow there, and each partial sum has a fixed place and is added in a fixed order, so the
-// norm does not depend on which wave is done first (no atomics).
+// norm is a function of the values, sizes and types alone: not of which wave is done first (no atomics) and not of addresses.
 //
 // What bounds it.  Memory, from some 10 MB on: a multiplication or two a value for the norm and clipping, some 60
 // instructions (a division and a root among them) for the update.  Measured on an MI355X, where a copy of 4 GiB runs at 4.8
@@ -514,18 +514,22 @@ int64_t total_bytes(int64_t count, const int64_t *numel, const int *dtype) {
     return n;
 }
 
+int64_t adam_bytes(int64_t count, const int64_t *numel, const int *dtype) {        // of all four tensors
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; i++) n += numel[i] * (kSize[dtype[i]] == 8 ? 32 : 8 + 2 * kSize[dtype[i]]);
+    return n;
+}
+
 // Puts tensors `from` to `to` of a call into a list: fill(place, tensor).  Empty ones have a place and no units.  Units begin at
-// cache lines of the tensor at `anchor` (of values of `size(i)` bytes): 402 tensors of a bucket, which begin anywhere, are
-// updated in 261 us for 281 us from their first values on.
-constexpr int kLine = 128;
-template <class List, class Anchor, class Size, class Fill>
-void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const int *dtype, int shift, Anchor anchor, Size size, Fill fill) {
+// the tensor's first value (head(i) of 0, for sums), or behind its first head(i) values, at a cache line.
+template <class List, class Head, class Fill>
+void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const int *dtype, int shift, Head head, Fill fill) {
     uint32_t units = 0;
     for (int64_t i = from; i < to; i++) {
         const int at = int(i - from);
-        const int64_t head = std::min<int64_t>(numel[i], (-uintptr_t(anchor[i]) & (kLine - 1)) / size(i));
-        if (numel[i]) units += uint32_t(std::max<int64_t>((numel[i] - head + (int64_t(1) << shift) - 1) >> shift, 1));
-        l.u.n[at] = uint64_t(numel[i]) << 8 | uint64_t(head) << 2 | uint64_t(dtype[i]);
+        const int64_t h = std::min<int64_t>(numel[i], head(i));
+        if (numel[i]) units += uint32_t(std::max<int64_t>((numel[i] - h + (int64_t(1) << shift) - 1) >> shift, 1));
+        l.u.n[at] = uint64_t(numel[i]) << 8 | uint64_t(h) << 2 | uint64_t(dtype[i]);
         l.u.end[at] = units;
         fill(at, i);
     }
@@ -533,6 +537,11 @@ void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const in
     l.u.shift = shift;
     l.u.units = units;
 }
+// Values of `size` bytes before the first cache line that begins in a tensor.  What is written is aligned to them: 402 tensors of
+// a bucket, which begin anywhere, are updated in 261 us for 281 us from their first values on.
+int64_t before_line(const void *p, int64_t size) { return int64_t(-uintptr_t(p) & 127) / size; }
+int64_t from_first(int64_t) { return 0; }
+
 template <class U> int grid_of(const U &u, int most = kMaxBlocks, int each = 1) {
     return int(std::min<int64_t>((int64_t(u.units) + kWaves * each - 1) / (kWaves * each), most));
 }
@@ -598,7 +607,13 @@ int launched(const char *what) {
     return report(-10, text);
 }
 
-// Workspace: [total, unused][partial sums][Scalars of each tensor]
+// Whether one block takes a list on alone.
+bool small(int op, int64_t count, const int64_t *numel, const int *dtype) {
+    if (op == MBRL_OP_ADAM) return count <= kSmallList && adam_bytes(count, numel, dtype) <= kSmallAdam;
+    return count <= kNormList && total_bytes(count, numel, dtype) <= (op == MBRL_OP_CLIP ? kSmallClip : kSmallNorm);
+}
+
+// Workspace of the others: [total, unused][partial sums][Scalars of each tensor]
 int64_t partials(int64_t count) { return (count + kNormList - 1) / kNormList * kMaxBlocks; }
 struct Space {
     double *total, *part;
@@ -608,25 +623,40 @@ struct Space {
         part = total + 2;
         scalars = reinterpret_cast<Scalars *>(part + partials(count));
     }
-    static int64_t bytes(int64_t count) { return 16 + 8 * partials(count) + int64_t(sizeof(Scalars)) * count; }
+    static int64_t bytes(int op, int64_t count, const int64_t *numel, const int *dtype) {
+        return small(op, count, numel, dtype) ? 0 : 16 + 8 * partials(count) + int64_t(sizeof(Scalars)) * count;
+    }
 };
 
-// The gradients of a call, for a norm or scaling, to which it is all one where a tensor ends: neighbours in memory of one type
-// become one.  A bucket of many tensors is one long run then, which takes one launch instead of one for each kNormList (402
-// tensors, 53 MB, clipped: 29 us for 50).
+// The gradients of a call.
 struct Gradients {
     int64_t count, values, bytes;
     void *const *x;
     const int64_t *numel;
     const int *dtype;
+    Gradients(int64_t count_, void *const *xs, const int64_t *ns, const int *types)
+        : count(count_), values(total(count_, ns)), bytes(total_bytes(count_, ns, types)), x(xs), numel(ns), dtype(types) {}
+
+    template <class L, class Head, class Go> void lists(L &l, int shift, Head head, Go go) const {
+        constexpr int K = decltype(l.u)::K;
+        l.u.count = l.u.units = 0;
+        for (int64_t i = 0; i < count; i += K) {
+            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head, [&](int at, int64_t k) { l.x[at] = x[k]; });
+            go();
+        }
+    }
+};
+
+// For scaling it is all one where a tensor ends: neighbours in memory of one type become one, and a bucket of many tensors takes
+// one launch instead of one for each kNormList.  Not for sums, whose order, and with it their last bit, must not hang on
+// where tensors lie: every rank of a sharded run clips by the same factor.
+struct Runs : Gradients {
     std::vector<void *> x_;
     std::vector<int64_t> numel_;
     std::vector<int> dtype_;
-
-    Gradients(int64_t count_, void *const *xs, const int64_t *ns, const int *types)
-        : count(count_), values(total(count_, ns)), bytes(total_bytes(count_, ns, types)), x(xs), numel(ns), dtype(types) {
+    explicit Runs(const Gradients &g) : Gradients(g) {
         auto follows = [&](int64_t i) {
-            return types[i] == types[i - 1] && ns[i - 1] && static_cast<char *>(xs[i - 1]) + ns[i - 1] * kSize[types[i]] == xs[i];
+            return g.dtype[i] == g.dtype[i - 1] && g.numel[i - 1] && static_cast<char *>(g.x[i - 1]) + g.numel[i - 1] * kSize[g.dtype[i]] == g.x[i];
         };
         int64_t runs = count ? 1 : 0;
         for (int64_t i = 1; i < count; i++) runs += !follows(i);
@@ -634,24 +664,15 @@ struct Gradients {
         x_.reserve(runs), numel_.reserve(runs), dtype_.reserve(runs);
         for (int64_t i = 0; i < count; i++) {
             if (i && follows(i)) {
-                numel_.back() += ns[i];
+                numel_.back() += g.numel[i];
                 continue;
             }
-            x_.push_back(xs[i]), numel_.push_back(ns[i]), dtype_.push_back(types[i]);
+            x_.push_back(g.x[i]), numel_.push_back(g.numel[i]), dtype_.push_back(g.dtype[i]);
         }
         count = runs;
         x = x_.data(), numel = numel_.data(), dtype = dtype_.data();
     }
-
-    template <class L, class Go> void lists(L &l, int shift, Go go) const {
-        constexpr int K = decltype(l.u)::K;
-        l.u.count = l.u.units = 0;
-        for (int64_t i = 0; i < count; i += K) {
-            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, x, [&](int64_t k) { return kSize[dtype[k]]; },
-                      [&](int at, int64_t k) { l.x[at] = x[k]; });
-            go();
-        }
-    }
+    Runs(const Runs &) = delete;
 };
 
 // Calls f(the flag as a constant).
@@ -680,7 +701,7 @@ Parts launch_partials(const Gradients &g, bool stream, bool finish, const Space 
     by_flag(stream, [&](auto stream_) {
         constexpr bool kStream = stream_;
         by_count<NormList, kNormList>(g.count, kStream, [&](auto l) {
-            g.lists(l, unit_shift(g.values), [&] {
+            g.lists(l, unit_shift(g.values), from_first, [&] {
                 if (const int grid = grid_of(l.u, kMaxBlocks, kStream ? 1 : kUnits)) {
                     hipLaunchKernelGGL((norm_partials<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
                     parts += grid;
@@ -697,26 +718,29 @@ void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm,
     by_norm(kind, [&](auto P_) {
         constexpr int P = P_;
         if constexpr (P != kNoClip) {
-            if (g.bytes <= (kClip ? kSmallClip : kSmallNorm) && g.count <= kNormList) {
+            if (small(kClip ? MBRL_OP_CLIP : MBRL_OP_NORM, g.count, g.numel, g.dtype)) {
                 by_count<NormList, kNormList>(g.count, false, [&](auto l) {
-                    g.lists(l, kSmallShift, [] {});
+                    g.lists(l, kSmallShift, from_first, [] {});
                     hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
                 });
                 return;
             }
             const bool stream = g.bytes > kCache / 4;
             const Parts sum = launch_partials<P>(g, g.bytes > (kClip ? kCache : kCache / 2), !kClip || stream, ws, norm, st);
-            if constexpr (kClip)
+            if constexpr (kClip) {
+                const Runs runs(g);
+                auto head = [&](int64_t i) { return before_line(runs.x[i], kSize[runs.dtype[i]]); };
                 by_flag(stream, [&](auto stream_) {
                     constexpr bool kStream = stream_;
-                    by_count<NormList, kNormList>(g.count, kStream, [&](auto l) {
-                        g.lists(l, !kStream ? unit_shift(g.values) : g.bytes == 2 * g.values ? kScaleShift16 : kScaleShift, [&] {
+                    by_count<NormList, kNormList>(runs.count, kStream, [&](auto l) {
+                        runs.lists(l, !kStream ? unit_shift(g.values) : g.bytes == 2 * g.values ? kScaleShift16 : kScaleShift, head, [&] {
                             if (const int grid = grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks, kUnits))
                                 hipLaunchKernelGGL((clip_scale<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, sum.part, sum.parts,
                                                    max_norm, norm);
                         });
                     });
                 });
+            }
         }
     });
 }
@@ -735,9 +759,10 @@ int guarded(const char *what, F &&f) {
 
 extern "C" {
 
-int64_t mbrl_optim_workspace_bytes(int64_t count) {
-    if (count < 0 || count > (int64_t(1) << 24)) return report(-6, "mbrl_optim_workspace_bytes: the number of tensors is out of range");
-    return Space::bytes(count);
+int64_t mbrl_optim_workspace_bytes(int op, int64_t count, const int64_t *numel, const int *dtype) {
+    if (int rc = check_list("mbrl_optim_workspace_bytes", count, numel, dtype)) return rc;
+    if (op != MBRL_OP_NORM && op != MBRL_OP_CLIP && op != MBRL_OP_ADAM) return report(-7, "mbrl_optim_workspace_bytes: unknown operator");
+    return Space::bytes(op, count, numel, dtype);
 }
 
 int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel, const int *dtype, int norm_type, void *workspace,
@@ -745,8 +770,9 @@ int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel
     return guarded("mbrl_grad_norm: failed", [&] {
         if (int rc = check_list("mbrl_grad_norm", count, numel, dtype)) return rc;
         if (norm_type < MBRL_NORM_INF || norm_type > MBRL_NORM_TWO) return report(-7, "mbrl_grad_norm: unknown norm type");
-        if (!norm || !workspace || (count && !grads)) return report(-1, "mbrl_grad_norm: null argument");
-        if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
+        const int64_t need = Space::bytes(MBRL_OP_NORM, count, numel, dtype);
+        if (!norm || (need && !workspace) || (count && !grads)) return report(-1, "mbrl_grad_norm: null argument");
+        if (workspace_bytes < need) return report(-8, "mbrl_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
             if (numel[i] && !grads[i]) return report(-1, "mbrl_grad_norm: null tensor");
         launch_norm<false>(norm_type, Gradients(count, const_cast<void *const *>(grads), numel, dtype), Space(workspace, count), 0.0, norm,
@@ -761,8 +787,9 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
         if (int rc = check_list("mbrl_clip_grad_norm", count, numel, dtype)) return rc;
         if (norm_type < MBRL_NORM_INF || norm_type > MBRL_NORM_TWO) return report(-7, "mbrl_clip_grad_norm: unknown norm type");
         if (!(max_norm >= 0.0)) return report(-7, "mbrl_clip_grad_norm: max_norm must not be negative");
-        if (!norm || !workspace || (count && !grads)) return report(-1, "mbrl_clip_grad_norm: null argument");
-        if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_clip_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
+        const int64_t need = Space::bytes(MBRL_OP_CLIP, count, numel, dtype);
+        if (!norm || (need && !workspace) || (count && !grads)) return report(-1, "mbrl_clip_grad_norm: null argument");
+        if (workspace_bytes < need) return report(-8, "mbrl_clip_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
         Ranges r;
         r.r.reserve(count);
         for (int64_t i = 0; i < count; i++) {
@@ -786,9 +813,10 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         if (clip && !(max_norm >= 0.0)) return report(-7, "mbrl_adam_step: max_norm must not be negative");
         if (!(beta_one >= 0.0 && beta_one < 1.0 && beta_two >= 0.0 && beta_two < 1.0)) return report(-7, "mbrl_adam_step: betas must be in [0, 1)");
         if (!(eps >= 0.0)) return report(-7, "mbrl_adam_step: eps must not be negative");
-        if (!workspace || (count && (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps || !lr || !weight_decay)))
+        const int64_t need = Space::bytes(MBRL_OP_ADAM, count, numel, dtype);
+        if ((need && !workspace) || (count && (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps || !lr || !weight_decay)))
             return report(-1, "mbrl_adam_step: null argument");
-        if (workspace_bytes < Space::bytes(count)) return report(-8, "mbrl_adam_step: workspace too small (mbrl_optim_workspace_bytes)");
+        if (workspace_bytes < need) return report(-8, "mbrl_adam_step: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
             if (!steps[i] || (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i])))
                 return report(-1, "mbrl_adam_step: null tensor");
@@ -809,13 +837,12 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         const Space ws(workspace, count);
         const Betas b{beta_one, beta_two, std::log1p(beta_one - 1.0), std::log1p(beta_two - 1.0), eps};        // b - 1 is exact from 0.5 on
         const int64_t values = total(count, numel);
-        int64_t bytes = 0;
-        for (int64_t i = 0; i < count; i++) bytes += numel[i] * (kSize[dtype[i]] == 8 ? 32 : 8 + 2 * kSize[dtype[i]]);
-        auto lists = [&](auto &l, int shift, auto fill, auto go) {
+        const int64_t bytes = adam_bytes(count, numel, dtype);
+        auto lists = [&](auto &l, int shift, auto head, auto fill, auto go) {
             constexpr int K = std::decay_t<decltype(l.u)>::K;
             l.u.count = l.u.units = 0;
             for (int64_t i = 0; i < count; i += K) {
-                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, exp_avgs, [&](int64_t k) { return kSize[dtype[k]] == 8 ? 8 : 4; },
+                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head,
                           [&](int at, int64_t k) { l.x[at] = grads[k]; fill(at, k); });
                 go(i);
             }
@@ -825,21 +852,22 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         by_norm(clip ? norm_type : kNoClip, [&](auto P_) {
             constexpr int P = P_;
             constexpr bool kClip = P != kNoClip;
-            if (bytes <= kSmallAdam && count <= kSmallList) {
+            if (small(MBRL_OP_ADAM, count, numel, dtype)) {
                 by_count<SmallList, kSmallList>(count, false, [&](auto l) {
-                    lists(l.l, kSmallShift, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
+                    lists(l.l, kSmallShift, from_first, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
                     hipLaunchKernelGGL((adam_small<P, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, b, decoupled, max_norm, norm);
                 });
                 return;
             }
             const bool stream = bytes > kCache / 4;
             const int shift = unit_shift(values);
+            auto head = [&](int64_t i) { return before_line(exp_avgs[i], kSize[dtype[i]] == 8 ? 8 : 4); };
             Parts sum{nullptr, 0};
             if (count <= kAdamList) {
                 by_flag(kClip && total_bytes(count, numel, dtype) > kCache, [&](auto stream_) {
                     constexpr bool kStream = kClip && stream_;
                     by_count<BeginList, kAdamList>(count, kStream, [&](auto l) {
-                        lists(l, shift, counters(l), [&](int64_t) {
+                        lists(l, shift, from_first, counters(l), [&](int64_t) {
                             const int grid = kClip ? std::max(grid_of(l.u), 1) : 1;
                             hipLaunchKernelGGL((adam_begin<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, decoupled,
                                                ws.scalars, ws.part);
@@ -862,7 +890,7 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             by_flag(stream, [&](auto stream_) {
                 constexpr bool kStream = stream_;
                 by_count<UpdateList, kAdamList>(count, kStream, [&](auto l) {
-                    lists(l, !kStream ? shift : bytes == 32 * values ? kAdamShift64 : kAdamShift, tensors(l), [&](int64_t i) {
+                    lists(l, !kStream ? shift : bytes == 32 * values ? kAdamShift64 : kAdamShift, head, tensors(l), [&](int64_t i) {
                         if (const int grid = std::max(grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks), kClip && i == 0 ? 1 : 0))        // one block at least writes the norm
                             hipLaunchKernelGGL((adam_update<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, ws.scalars + i,
                                                sum.part, sum.parts, max_norm, norm);

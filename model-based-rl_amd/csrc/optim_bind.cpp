@@ -131,8 +131,9 @@ void type_of(const List &l, size_t i, Sizes &s) {
 struct Call {
     c10::OptionalDeviceGuard guard;
     at::Tensor norm, space;
+    int64_t bytes;
     void *stream;
-    Call(c10::Device dev, int64_t count, bool with_norm) {
+    Call(int op, c10::Device dev, const Sizes &s, bool with_norm) {
         if (dev.type() != c10::DeviceType::CUDA) {        // an empty list: the current GPU
             c10::impl::VirtualGuardImpl impl(c10::DeviceType::CUDA);
             if (impl.deviceCount() < 1) raise(mbrl_error, "no GPU visible: these operators run only on the HIP device (no CPU path)");
@@ -140,11 +141,12 @@ struct Call {
         }
         guard.reset_device(dev);
         stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
-        const int64_t bytes = workspace_bytes(count);
+        bytes = workspace_bytes(op, s.numel.size(), s.numel.data(), s.dtype.data());
         if (bytes < 0) raise(mbrl_error, last_error());
-        space = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+        if (bytes) space = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
         if (with_norm) norm = at::empty({}, at::TensorOptions().dtype(at::kDouble).device(dev));
     }
+    void *space_ptr() const { return space.defined() ? space.data_ptr() : nullptr; }
     double *norm_ptr() const { return norm.defined() ? static_cast<double *>(norm.data_ptr()) : nullptr; }
     PyObject *result() const {
         if (norm.defined()) return THPVariable_Wrap(norm);
@@ -259,8 +261,8 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
             type_of(g, i, s);
         }
         at.settle();
-        Call c(at.device, g.t.size(), true);
-        done(grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, c.space.data_ptr(), c.space.numel(), c.norm_ptr(), c.stream));
+        Call c(MBRL_OP_NORM, at.device, s, true);
+        done(grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, c.space_ptr(), c.bytes, c.norm_ptr(), c.stream));
         return c.result();
     });
 }
@@ -279,8 +281,8 @@ PyObject *py_clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
             type_of(g, i, s);
         }
         at.settle();
-        Call c(at.device, g.t.size(), true);
-        done(clip_grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, most, c.space.data_ptr(), c.space.numel(),
+        Call c(MBRL_OP_CLIP, at.device, s, true);
+        done(clip_grad_norm(g.t.size(), g.ptr.data(), s.numel.data(), s.dtype.data(), kind, most, c.space_ptr(), c.bytes,
                             c.norm_ptr(), c.stream));
         for (const at::Tensor *x : g.t) written(*x);
         return c.result();
@@ -325,11 +327,11 @@ PyObject *py_adam_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
             t.check(i, at);
         }
         at.settle();
-        Call c(at.device, count, clip);
+        Call c(MBRL_OP_ADAM, at.device, s, clip);
         std::vector<float *> steps(count);
         for (size_t i = 0; i < count; i++) steps[i] = static_cast<float *>(t.ptr[i]);
         done(adam_step(count, p.ptr.data(), g.ptr.data(), m.ptr.data(), v.ptr.data(), steps.data(), s.numel.data(), s.dtype.data(), lr.data(),
-                       wd.data(), b1, b2, eps, decoupled, kind, most, c.space.data_ptr(), c.space.numel(), c.norm_ptr(), c.stream));
+                       wd.data(), b1, b2, eps, decoupled, kind, most, c.space_ptr(), c.bytes, c.norm_ptr(), c.stream));
         for (const List *l : {&p, &m, &v, &t})
             for (const at::Tensor *x : l->t) written(*x);
         return c.result();

@@ -61,7 +61,7 @@ def load():
     L.mbrl_fd_plan_finish.argtypes = [vp, C.c_int64, vp, vp, C.c_int64, vp]
     L.mbrl_rollout_record.argtypes = [vp, C.c_int64, C.c_int] + [vp] * 5 + [vp, C.c_int64, C.c_int64, C.c_int64, vp]
     ppv, pi64, pint, pf64 = C.POINTER(vp), C.POINTER(C.c_int64), C.POINTER(C.c_int), C.POINTER(C.c_double)
-    L.mbrl_optim_workspace_bytes.argtypes = [C.c_int64]
+    L.mbrl_optim_workspace_bytes.argtypes = [C.c_int, C.c_int64, pi64, pint]
     L.mbrl_optim_workspace_bytes.restype = C.c_int64
     L.mbrl_grad_norm.argtypes = [C.c_int64, ppv, pi64, pint, C.c_int, vp, C.c_int64, vp, vp]
     L.mbrl_clip_grad_norm.argtypes = [C.c_int64, ppv, pi64, pint, C.c_int, C.c_double, vp, C.c_int64, vp, vp]

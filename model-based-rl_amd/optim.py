@@ -42,7 +42,8 @@ def bind():
 
 def grad_norm(grads, norm_type=2.0):
     """Norm over all values of all tensors in `grads` as a 0-d float64 tensor, summed in float64.  norm_type 1, 2 or inf.
-    0 for an empty list, NaN if any value is NaN."""
+    0 for an empty list, NaN if any value is NaN.  The same values in tensors of the same sizes give the same bits wherever
+    they lie, so ranks that hold the same gradients find the same norm."""
     return (_bind or bind()).grad_norm(grads, norm_type)
 
 
@@ -53,7 +54,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
     changed instead (it waits for the device, so not under graph capture).  Tensors that share memory are refused."""
     b = _bind or bind()
     if error_if_nonfinite:
-        if torch.cuda.is_current_stream_capturing():
+        grads = grads if isinstance(grads, torch.Tensor) else tuple(grads)        # an iterator would be empty the second time
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise ValueError("clip_grad_norm_: error_if_nonfinite waits for the device and cannot be captured into a graph")
         norm = float(b.grad_norm(grads, norm_type))
         if not math.isfinite(norm):
@@ -93,6 +95,8 @@ class FusedAdam(torch.optim.Optimizer):
             raise ValueError("FusedAdam: eps must not be negative, got %r" % (eps,))
         if max_norm is not None and not max_norm >= 0.0:
             raise ValueError("FusedAdam: max_norm must not be negative, got %r" % (max_norm,))
+        if norm_type not in (1, 2, math.inf):
+            raise ValueError("FusedAdam: norm_type has to be 1, 2 or inf, got %r" % (norm_type,))
         self.max_norm, self.norm_type, self.grad_norm = max_norm, norm_type, None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       decoupled_weight_decay=bool(decoupled_weight_decay)))

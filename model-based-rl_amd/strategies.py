@@ -263,7 +263,8 @@ class VariationalOptimization(nn.Module):
         is the 1-GPU gradient for the objective loss `R` (batch mean of per-step losses, :204); the REINFORCE
         baselines of PR / IR / SIR are then per-shard statistics.
         SOLVER.CLIP_GRAD_NORM > 0 bounds the global norm of the (summed) gradient before the step -- differences through
-        contacts grow with the horizon -- and adds it, as it was before clipping, to the returned statistics."""
+        contacts grow with the horizon -- and adds it, as it was before clipping, to the returned statistics.  Every rank
+        finds the same norm for the same summed gradient, so the ranks' parameters stay the same."""
         loss, stats = self.loss_functions.get(self.method, self.R_loss)(batch_loss)
         if self.local_batch != self.batch_size:
             loss = loss * (float(self.local_batch) / float(self.batch_size))
@@ -273,12 +274,12 @@ class VariationalOptimization(nn.Module):
         if grad_sync is not None:
             grad_sync(grads)
         max_norm, norm = float(self.cfg.SOLVER.CLIP_GRAD_NORM), None
-        if max_norm > 0 and not self.cfg.SOLVER.FUSED:
+        if max_norm and not self.cfg.SOLVER.FUSED:
             norm = optim.clip_grad_norm_(grads, max_norm)
         if self.cfg.SOLVER.OPTIMIZER == "sgd":
             nn.utils.clip_grad_value_(self.parameters(), 1)
         self.optimizer.step()
-        if max_norm > 0:
+        if max_norm:
             stats["grad_norm"] = float(self.optimizer.grad_norm if norm is None else norm)
         with torch.no_grad():                      # "Make sure sd is not negative" :357-359
             self.sd.data.clamp_(min=self.sd_threshold)

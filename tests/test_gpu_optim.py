@@ -391,6 +391,7 @@ def test_captured_and_replayed():
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         with pytest.raises(ValueError, match="captured"):
             optim.clip_grad_norm_(eager[1], 1.0, error_if_nonfinite=True)
+        optim.grad_norm(eager[1])
 
 
 def test_streams_beside_each_other():
@@ -408,6 +409,33 @@ def test_streams_beside_each_other():
         assert abs(float(n[0]) - ref_norm(a, 2)) <= norm_tol(a) * ref_norm(a, 2)
         # clipped once: under the bound from then on, but for the rounding of 2e5 values
         assert abs(float(n[1]) - 1.0) < 2e-6 and float(n[2]) <= 1.0 + 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_does_not_hang_on_addresses(dtype):
+    """The same values in tensors of their own, one behind another, at odd places and in any dense order: the same bits, so that
+    all ranks of a sharded run clip by the same factor."""
+    torch, optim = _t()
+    for sizes in ([(700,), (3, 5), (0,), (4097,), (512,), (64, 64)], [(1 + 997 * i % 4000,) for i in range(300)], [(1 << 20,), (70001,), (1,)]):
+        apart = make(sizes, [dtype], seed=75)
+        n = sum(t.numel() for t in apart)
+        results = []
+        for lead in (0, 1, 7):
+            buf = torch.zeros(n + lead, dtype=apart[0].dtype, device="cuda")[lead:]
+            views = [v.view(t.shape) for v, t in zip(buf.split([t.numel() for t in apart]), apart)]
+            results.append([v.copy_(t) for v, t in zip(views, apart)])
+        for p in (1, 2):
+            want = float(optim.grad_norm(apart, p))
+            assert all(float(optim.grad_norm(v, p)) == want for v in results)
+        want = float(optim.clip_grad_norm_([t.clone() for t in apart], 1.0))
+        adam = lambda ts: float(optim.adam_step([t.clone() for t in ts], ts, *[[torch.zeros(t.shape, dtype=torch.float64 if dtype == "float64"    # noqa: E731
+                                 else torch.float32, device="cuda") for t in ts] for _ in range(2)],
+                                [torch.zeros((), device="cuda") for _ in ts], 0.0, max_norm=1.0))
+        first = adam(apart)
+        for v in results:
+            assert adam(v) == first and float(optim.clip_grad_norm_(v, 1.0)) == want
+        for v in results[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(v, results[0]))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -533,6 +561,105 @@ def test_a_run_of_them_together():
         # an entry of Adam's step is at most lr (1 - b1) / sqrt(1 - b2) = 3.2 lr: where a gradient's sign is rounding, the two differ by twice that
         off = torch.cat([(p.detach().double().cpu() - q.detach()).abs().reshape(-1) for p, q in zip(net.parameters(), ref.parameters())])
         assert float(off.max()) <= 2 * 3.2e-3 and float(off.median()) <= 1e-5
+
+
+def test_fused_adam_captured():
+    """A captured step() counts its steps on the device: replays follow eager steps bit for bit, with other gradients each time."""
+    torch, optim = _t()
+    sizes = [(40, 30), (30,), (6, 40)]
+    eager, graphed = ([t.clone().requires_grad_() for t in make(sizes, ["float32", "float32", "float64"], 81)] for _ in range(2))
+    opts = [optim.FusedAdam(l, 0.01, weight_decay=0.01, max_norm=1.5) for l in (eager, graphed)]
+    for l in (eager, graphed):
+        for p in l:
+            p.grad = torch.zeros_like(p)
+    opts[1].step()                        # makes the state outside the capture
+    opts[0].step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[1].step()
+    norm = opts[1].grad_norm
+    for k in range(4):
+        for p, q, g in zip(eager, graphed, make(sizes, ["float32", "float32", "float64"], 90 + k)):
+            p.grad.copy_(g)
+            q.grad.copy_(g)
+        opts[0].step()
+        graph.replay()
+        float(optim.grad_norm([p.grad for p in eager]))
+        assert float(norm) == float(opts[0].grad_norm)
+        for p, q in zip(eager, graphed):
+            assert torch.equal(p, q) and torch.equal(opts[0].state[p]["exp_avg_sq"], opts[1].state[q]["exp_avg_sq"])
+            assert float(opts[1].state[q]["step"]) == k + 2
+
+
+def test_fused_adam_saves_and_goes_on():
+    """16-bit parameters with their float32 moments, many of them: saved, loaded into a new optimiser, the same bits from there on.
+    A closure, a scheduler, and a parameter of permuted dimensions on the way."""
+    torch, optim = _t()
+    sizes = [(11, 7, 5)] + [(3 * i % 50,) for i in range(120)]
+
+    def params():
+        ps = [t.clone().requires_grad_() for t in make(sizes, ["bfloat16", "float16", "float32"], 101)]
+        ps[0] = ps[0].detach().permute(2, 0, 1).contiguous().permute(1, 2, 0).requires_grad_()
+        return ps
+
+    def run(ps, opt, sched, ks):
+        for k in ks:
+            gs = make(sizes, ["bfloat16", "float16", "float32"], 200 + k)
+
+            def closure():
+                for p, g in zip(ps, gs):
+                    p.grad = torch.empty_like(p).copy_(g)       # laid out like its parameter, as autograd leaves it
+                return k
+            assert opt.step(closure) == k
+            sched.step()
+    a, b = params(), params()
+    one = optim.FusedAdam(a, 0.05, max_norm=3.0, norm_type=1, weight_decay=0.1, decoupled_weight_decay=True)
+    sa = torch.optim.lr_scheduler.StepLR(one, 1, 0.5)
+    run(a, one, sa, range(6))
+    first = optim.FusedAdam(b, 0.05, max_norm=3.0, norm_type=1, weight_decay=0.1, decoupled_weight_decay=True)
+    sb = torch.optim.lr_scheduler.StepLR(first, 1, 0.5)
+    run(b, first, sb, range(3))
+    second = optim.FusedAdam(b, 1.0, max_norm=3.0, norm_type=1)
+    sc = torch.optim.lr_scheduler.StepLR(second, 1, 0.5)
+    second.load_state_dict(first.state_dict())
+    sc.load_state_dict(sb.state_dict())
+    run(b, second, sc, range(3, 6))
+    assert one.param_groups[0]["lr"] == second.param_groups[0]["lr"] == pytest.approx(0.05 / 64)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and torch.equal(one.state[p]["exp_avg"], second.state[q]["exp_avg"])
+    assert one.state[a[0]]["exp_avg"].stride() == a[0].stride() and one.state[a[0]]["exp_avg"].dtype == torch.float32
+    with pytest.raises(ValueError, match="another order"):
+        a[0].grad = torch.zeros((11, 7, 5), dtype=a[0].dtype, device="cuda")
+        one.step()
+
+
+def test_threads_and_inference_tensors():
+    torch, optim = _t()
+    import threading
+    lists = [make([(30011,), (5,), (700,)], ["float32", "float64"], 300 + i) for i in range(4)]
+    want = [host(l) for l in lists]
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got[i] = float(optim.grad_norm(lists[i]))
+                with pytest.raises(ValueError, match="norm_type"):
+                    optim.grad_norm(lists[i], 5)
+        except Exception as e:          # noqa: BLE001
+            errors.append(e)
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not errors
+    for g, a in zip(got, want):
+        assert abs(g - ref_norm(a, 2)) <= norm_tol(a) * ref_norm(a, 2)
+    with torch.inference_mode():
+        x = torch.full((64,), 2.0, device="cuda")
+        assert float(optim.clip_grad_norm_([x], 8.0)) == 16.0
+    assert float(x[3]) == pytest.approx(1.0)
 
 
 @pytest.mark.parametrize("fused", [False, True])

@@ -39,6 +39,7 @@ def test_no_cpu_path():
     (lambda: optim.grad_norm([Z(4, 6)[:, :3]]), ValueError, "gaps"),
     (lambda: optim.grad_norm([Z(1).expand(5)]), ValueError, "repeated"),
     (lambda: optim.grad_norm([torch._neg_view(Z(3))]), ValueError, "negated"),
+    (lambda: optim.clip_grad_norm_(Z(3), 1.0, error_if_nonfinite=True), TypeError, "a list"),
     (lambda: optim.clip_grad_norm_([Z(3)], -1.0), ValueError, "max_norm"),
     (lambda: optim.clip_grad_norm_([Z(3)], math.nan), ValueError, "max_norm"),
     (lambda: optim.clip_grad_norm_([Z(8)[::2]], 1.0), ValueError, "gaps"),
@@ -87,15 +88,18 @@ def test_abi_refusals():
     """Addresses here are numbers that nothing follows: every call is refused before a launch."""
     L = lib.load()
     ws, norm = C.c_void_p(0x1000), C.c_void_p(0x8000)
-    big = L.mbrl_optim_workspace_bytes(4)
-    assert 0 < L.mbrl_optim_workspace_bytes(0) <= big < L.mbrl_optim_workspace_bytes(500)
-    assert L.mbrl_optim_workspace_bytes(-1) == -6
+    need = lambda op, l: L.mbrl_optim_workspace_bytes(op, l[0], l[2], l[3])      # noqa: E731
+    long = _arrays([0x1000000 * (i + 1) for i in range(3)], [100000] * 3, [1] * 3)
+    big = need(2, long)
+    assert big > 0 and need(0, _arrays([], [], [])) == 0 and need(0, _arrays([1], [16], [1])) == 0
+    assert need(2, _arrays([0] * 500, [1 << 20] * 500, [2] * 500)) > big
+    assert need(3, long) == -7 and L.mbrl_optim_workspace_bytes(0, -1, None, None) == -6 and L.mbrl_optim_workspace_bytes(0, 2, None, None) == -1
     clip = lambda l, most=1.0, kind=2, w=ws, b=big, out=norm: L.mbrl_clip_grad_norm(*l, kind, most, w, b, out, None)   # noqa: E731
     good = _arrays([0x10000, 0x20000], [16, 16], [1, 1])
     assert clip(good, kind=3) == -7 and b"norm type" in L.mbrl_last_error()
     assert clip(good, most=-1.0) == -7 and clip(good, most=math.nan) == -7
-    assert clip(good, b=big // 8) == -8 and b"workspace" in L.mbrl_last_error()
-    assert clip(good, w=None) == -1 and clip(good, out=None) == -1
+    assert clip(long, b=need(1, long) - 1) == -8 and b"workspace" in L.mbrl_last_error()
+    assert clip(long, w=None) == -1 and clip(good, out=None) == -1
     assert clip(_arrays([0x10000, None], [16, 16], [1, 1])) == -1
     assert clip(_arrays([0x10000], [-1], [1])) == -6 and clip(_arrays([0x10000], [1 << 41], [1])) == -6
     assert clip(_arrays([0x10000], [16], [4])) == -7 and clip(_arrays([0x10000], [16], [-1])) == -7
@@ -109,7 +113,7 @@ def test_abi_refusals():
     def adam(params=0x10000, grads=0x20000, avgs=0x30000, sqs=0x40000, steps=0x50000, b1=0.9, b2=0.999, eps=1e-8, bytes_=big):
         return L.mbrl_adam_step(1, p(params), p(grads), p(avgs), p(sqs), p(steps), one, (C.c_int * 1)(1), f64, f64, b1, b2, eps, 0, 2,
                                 1.0, ws, bytes_, None, None)
-    assert adam(b1=1.0) == -7 and adam(b2=-0.1) == -7 and adam(b1=math.nan) == -7 and adam(eps=-1.0) == -7 and adam(bytes_=8) == -8
+    assert adam(b1=1.0) == -7 and adam(b2=-0.1) == -7 and adam(b1=math.nan) == -7 and adam(eps=-1.0) == -7
     assert adam(steps=None) == -1 and adam(grads=None) == -1
     for over in (dict(avgs=0x10000), dict(sqs=0x30000), dict(grads=0x10020), dict(steps=0x40004)):
         assert adam(**over) == -7 and b"shares memory" in L.mbrl_last_error(), over
@@ -117,14 +121,14 @@ def test_abi_refusals():
     n = 70000
     many = _arrays([0x100000 + 64 * ((i * 7919) % n) for i in range(n)], [16] * n, [1] * n)
     many[1][n - 1] = many[1][0]
-    assert clip(many, b=L.mbrl_optim_workspace_bytes(n)) == -7 and b"share memory" in L.mbrl_last_error()
+    assert clip(many, b=need(1, many)) == -7 and b"share memory" in L.mbrl_last_error()
     # gradients are only read: two parameters may have the same one, and the norm may count a tensor twice
     assert L.mbrl_grad_norm(*good, 5, ws, big, norm, None) == -7
 
 
 def test_fused_adam_construction_and_state_dict():
     p = [torch.nn.Parameter(Z(3)), torch.nn.Parameter(Z(2, 2, dtype=torch.bfloat16))]
-    for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(max_norm=-1.0)):
+    for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(max_norm=-1.0), dict(norm_type=3)):
         with pytest.raises(ValueError):
             optim.FusedAdam(p, **bad)
     opt = optim.FusedAdam([{"params": [p[0]], "lr": 0.1}, {"params": [p[1]], "betas": (0.5, 0.9)}])
@@ -204,5 +208,9 @@ def test_strategy_clips_the_summed_gradient_before_the_step(solver, monkeypatch)
         want = before[0] - 0.5 * 0.25 * torch.ones_like(before[0]) / math.sqrt(5)
         assert torch.allclose(pol.mean.detach(), want, rtol=0, atol=1e-6)
     calls.clear()
+    monkeypatch.undo()
+    cfg.SOLVER.CLIP_GRAD_NORM = -1.0
+    with pytest.raises(ValueError, match="max_norm"):
+        pol.optimize((pol.mean.sum() * 3.0).expand(4, 5) + 0 * pol.sd.sum())
     cfg.SOLVER.CLIP_GRAD_NORM = 0.0
     assert "grad_norm" not in pol.optimize((pol.mean.sum() * 3.0).expand(4, 5) + 0 * pol.sd.sum()) and not calls
