@@ -16,14 +16,14 @@
 //
 // What bounds it.  Memory, from some 10 MB on: a multiplication or two a value for the norm and clipping, some 60
 // instructions (a division and a root among them) for the update.  Measured on an MI355X, where a copy of 4 GiB runs at 4.8
-// TB/s and x *= c at 5.9, float32 values, kernel arguments and all launches included:
-//   values            norm                 clip (scaled)          Adam                  Adam, clipped
-//   8e3               3.7 us               5.5 us                 6.2 us                8.4 us           one launch
-//   5e5               4.8 us               6.8 us                 6.2 us                8.3 us           two launches
-//   8e6               6.5 us, 5.0 TB/s     13.6 us, 7.0 TB/s      41 us, 5.5 TB/s       48 us            from the cache
-//   268e6             161 us, 6.6 TB/s     517 us, 6.2 TB/s       1.23 ms, 6.1 TB/s     1.39 ms          from memory
+// TB/s and x *= c at 5.9, 10 float32 tensors of as many values in all, every launch included:
+//   values    norm               clip (scaled)       Adam                Adam, clipped
+//   8e3       3.5 us             5.1 us              6.2 us              8.1 us         one launch
+//   5e5       4.9 us             6.7 us              6.1 us              7.9 us         two launches
+//   8e6       6.6 us, 4.9 TB/s   14.7 us, 6.5 TB/s   39 us, 5.7 TB/s     46 us          from the cache
+//   268e6     164 us, 6.5 TB/s   525 us, 6.1 TB/s    1.23 ms, 6.1 TB/s   1.40 ms        from memory
 // (clip: two reads and a write).  Below that it is the launches: an empty one takes 2.2 us of the device and 3.7 us of the
-// host, so small lists are done in one.
+// host, so small lists are done in one (a call of 2 or 10 tensors: 4.3 us of the host for a norm).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -43,8 +43,8 @@ using mbrl::report;
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 
 // Bytes that one block of 16 waves takes on alone, in one launch (of gradients; of all four tensors for Adam).  Against the two
-// launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.9 / 5.3 for 4.6 / 8.1, clipping of
-// 24e3 6.9 / 7.1 for 6.0 / 8.7, Adam of 12e3 7.2 / 7.5 for 5.5 / 9.0.  Twice as much is slower both ways for the last two.
+// launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.7 / 5.0 for 4.6 / 8.1, clipping of
+// 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 11e3 6.5 / 6.8 for 5.5 / 9.0.  Twice as much is slower both ways for the last two.
 constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
 constexpr int kSmallShift = 8;            // units of one 1 KB load a wave: 800-value tensors 6.6 us for 7.2 with twice that (Adam)
