@@ -221,11 +221,14 @@ def adam_bounds(x, g, m, v, t, lr, b1, b2, eps, wd, decoupled, c, u, c_err):
     g1 = c g: factor rounded, product: 2u (and the factor's own error).  L2: wd rounded, one fused product: 2u |wd x| + u |g1|.
     m': a1 = 1 - b1 rounded, a1 g1 rounded, b1 rounded, one fused sum.
     v': a2 rounded, two products, g1 squared (twice its error); b2 rounded; one fused sum.
-    d = sqrt(v') root + eps: half of v's error, sqrt, root and eps rounded, one fused sum.
-    x' = x keep - size (m' / d): quotient, size, keep, product, one fused sum.
+    d = sqrt(v') root + eps: half of v's error, sqrt, root and eps rounded, one fused sum.  A float32 root may be the hardware's
+    own, within a step (2 u) instead of half a one, of an argument that may have been scaled by a power of 2.
+    x' = x keep - size (m' / d): quotient, size, keep, product, one fused sum.  A float32 quotient may be the product with the
+    hardware's reciprocal: a step (2 u) and the product's rounding (u) instead of u.
     size and root come from 1 - b^t = -expm1(t log1p(b - 1)) in float64: log1p and expm1 within a step (2 w with w = 2^-53), the
     product w, and expm1 of a negative number passes on at most its argument's relative error: 5 w, a division (and a root)
     more: 6 w.  keep = 1 - lr wd: two roundings."""
+    own = 2 if u == 2.0 ** -24 else 0        # u more in a float32 quotient, half of that in a root
     x, g, m, v = (a.astype(np.longdouble) for a in (x, g, m, v))
     b1, b2, one, w = np.longdouble(b1), np.longdouble(b2), np.longdouble(1), 2.0 ** -53
     g1 = np.longdouble(c) * g
@@ -239,12 +242,12 @@ def adam_bounds(x, g, m, v, t, lr, b1, b2, eps, wd, decoupled, c, u, c_err):
     ev = 2 * u * b2 * v + (1 - b2) * (2 * np.abs(g1) * eg + eg * eg + 4 * u * g1 * g1) + u * v1
     root = one / np.sqrt(one - b2 ** t)
     s = np.sqrt(v1)
-    es = np.where(v1 > 0, ev / (2 * np.where(v1 > 0, s, 1)), np.sqrt(ev)) + u * s
+    es = np.where(v1 > 0, ev / (2 * np.where(v1 > 0, s, 1)), np.sqrt(ev)) + (1 + own / 2) * u * s
     d = s * root + eps
     ed = es * root + (3 * u + 6 * w) * s * root + u * eps + u * d
     size = lr / (one - b1 ** t)
     q = m1 / d
-    eq = em / d + np.abs(q) * ed / d + u * np.abs(q)
+    eq = em / d + np.abs(q) * ed / d + (1 + own) * u * np.abs(q)
     keep = one - np.longdouble(lr) * np.longdouble(wd) if decoupled else one
     x1 = x * keep - size * q
     ex = size * eq + (2 * u + 6 * w) * size * np.abs(q) + 3 * u * np.abs(x * keep) * (1 if decoupled else 0) + u * np.abs(x1)
@@ -306,6 +309,29 @@ def test_adam_list_borders(count):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_adam_of_one_tensor(n, dtype):
     check_adam([(n,)], [dtype], 0.5)
+
+
+def test_adam_of_the_smallest_and_largest_moments():
+    """Second moments from nothing and subnormal values to the largest, with and without eps, against float64.  m, v, root, scale,
+    sum, quotient, size and product: 12 half steps at most."""
+    torch, optim = _t()
+    v = torch.tensor([0.0, 1e-45, 3e-42, 1e-38, 2e-30, 1e-12, 1.0, 1e20, 3e38], device="cuda")
+    for eps in (0.0, 1e-8):
+        for n in (9, 300001):
+            vs = v.repeat(n // 9 + 1)[:n].contiguous()
+            m = torch.full((n,), 1e-3, device="cuda")
+            x, g, t = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.full((), 9.0, device="cuda")
+            want_v = vs.double().cpu().numpy() * float(np.float32(0.99))
+            want_v = want_v.astype(np.float32).astype(np.float64)          # one rounding, of subnormal values too
+            optim.adam_step([x], [g], [m], [vs], [t], 0.5, (0.9, 0.99), eps)
+            assert np.array_equal(vs.double().cpu().numpy(), want_v)
+            m1 = m.double().cpu().numpy()
+            d = np.sqrt(want_v) / math.sqrt(1 - 0.99 ** 10) + eps
+            with np.errstate(divide="ignore"):
+                want = -0.5 / (1 - 0.9 ** 10) * m1 / d
+            got = x.double().cpu().numpy()
+            big = np.abs(want) > 3e38
+            assert np.all(np.isinf(got[big]) & (got[big] < 0)) and np.all(np.abs(got[~big] - want[~big]) <= 12 * 2.0 ** -24 * np.abs(want[~big]) + 1e-37)
 
 
 def test_adam_keeps_infinite_parameters_apart_from_their_moments():
