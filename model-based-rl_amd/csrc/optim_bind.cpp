@@ -186,13 +186,13 @@ std::vector<double> numbers(PyObject *o, size_t n, const char *name) {
         if (!std::isfinite(v) || v < 0.0) raise(PyExc_ValueError, std::string(name) + " must be finite and not negative");
         return std::vector<double>(n, v);
     }
-    PyObject *seq = PySequence_Fast(o, "expected a number or a list of numbers");
+    PyObject *seq = PySequence_Tuple(o);        // of its own, as List's
     if (!seq) throw Raised{};
     std::vector<double> out;
-    bool ok = size_t(PySequence_Fast_GET_SIZE(seq)) == n, fits = true;
+    bool ok = size_t(PyTuple_GET_SIZE(seq)) == n, fits = true;
     out.reserve(n);
     for (size_t i = 0; ok && i < n; i++) {
-        const double v = PyFloat_AsDouble(PySequence_Fast_GET_ITEM(seq, i));
+        const double v = PyFloat_AsDouble(PyTuple_GET_ITEM(seq, i));
         if (v == -1.0 && PyErr_Occurred()) {
             Py_DECREF(seq);
             throw Raised{};

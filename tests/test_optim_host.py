@@ -79,6 +79,17 @@ def test_refused_adam_steps(over, error, text):
         _adam(**over)
 
 
+def test_a_list_of_rates_that_changes_while_it_is_read():
+    class Shrinks:
+        def __float__(self):
+            rates.clear()
+            return 1e-3
+    rates = [Shrinks()] + [1e-3] * 63
+    n = len(rates)
+    with pytest.raises(lib.MbrlError, match="no CPU path"):
+        optim.adam_step(*([Z(2) for _ in range(n)] for _ in range(4)), [Z(()) for _ in range(n)], rates)
+
+
 def _arrays(ptrs, numel, dtype):
     n = len(ptrs)
     return n, (C.c_void_p * n)(*ptrs), (C.c_int64 * n)(*numel), (C.c_int * n)(*dtype)
