@@ -370,7 +370,9 @@ __global__ __launch_bounds__(kSmallThreads) void norm_small(const L l, double ma
 }
 
 // ---- Adam ----
-struct Betas { double b1, b2, log_b1, log_b2, eps; };
+// up: a power of 2 that root, eps and with them the denominator are multiplied by, and size for it, so that an eps near the
+// ends of float32 has a normal reciprocal there (scale_of()).
+struct Betas { double b1, b2, log_b1, log_b2, eps, up; };
 
 // Counts a tensor's step and turns it into what the update multiplies with, in float64.
 __device__ __forceinline__ Scalars count_step(float *count, double lr, double wd, const Betas &b, int decoupled) {
@@ -378,8 +380,8 @@ __device__ __forceinline__ Scalars count_step(float *count, double lr, double wd
     *count = step;
     const double t = step;
     Scalars s;
-    s.size = lr / -expm1(t * b.log_b1);        // 1 - b^t without the cancellation
-    s.root = 1.0 / sqrt(-expm1(t * b.log_b2));
+    s.size = b.up * lr / -expm1(t * b.log_b1);        // 1 - b^t without the cancellation
+    s.root = b.up / sqrt(-expm1(t * b.log_b2));
     s.keep = decoupled ? 1.0 - lr * wd : 1.0;
     s.l2 = decoupled ? 0.0 : wd;
     return s;
@@ -566,6 +568,10 @@ void by_norm(int kind, F &&f) {
     else if (kind == MBRL_NORM_INF) f(std::integral_constant<int, MBRL_NORM_INF>{});
     else f(std::integral_constant<int, kNoClip>{});
 }
+
+// The denominator lies between eps and the largest float32 root, 2^64, times its scale, at most 2^27.  The hardware's reciprocal
+// takes a subnormal denominator for 0 and gives 0 where it would be subnormal itself, beyond 2^126: 1 will do in between.
+double scale_of(double eps) { return eps > 0.0 && eps < 0x1p-126 ? 0x1p32 : eps >= 0x1p64 ? 0x1p-64 : 1.0; }
 
 constexpr int64_t kMaxValues = int64_t(1) << 37;        // of a call: units are counted in 32 bits
 
@@ -848,7 +854,8 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
         if (!r.disjoint()) return report(-7, "mbrl_adam_step: a tensor that is written shares memory with another one");
         const hipStream_t st = (hipStream_t)hip_stream;
         const Space ws(workspace, count);
-        const Betas b{beta_one, beta_two, std::log1p(beta_one - 1.0), std::log1p(beta_two - 1.0), eps};        // b - 1 is exact from 0.5 on
+        const double up = scale_of(eps);
+        const Betas b{beta_one, beta_two, std::log1p(beta_one - 1.0), std::log1p(beta_two - 1.0), up * eps, up};        // b - 1 is exact from 0.5 on
         const int64_t values = total(count, numel);
         const int64_t bytes = adam_bytes(count, numel, dtype);
         auto lists = [&](auto &l, int shift, auto head, auto fill, auto go) {

@@ -334,6 +334,27 @@ def test_adam_of_the_smallest_and_largest_moments():
             assert np.all(np.isinf(got[big]) & (got[big] < 0)) and np.all(np.abs(got[~big] - want[~big]) <= 12 * 2.0 ** -24 * np.abs(want[~big]) + 1e-37)
 
 
+@pytest.mark.parametrize("eps", [2.0 ** -149, 1e-40, 1e-38, 2e-38, 1e20, 1e38, 2.0 ** 127])
+def test_adam_with_an_eps_at_the_ends_of_float32(eps):
+    """An eps whose reciprocal is subnormal or infinite, or that is subnormal itself, over second moments that leave it alone in
+    the denominator or not.  Roundings as in adam_bounds(): root 2 (in half steps), its scale, eps and the sum 1 each,
+    quotient 3, size and product 1 each: 10."""
+    torch, optim = _t()
+    m0 = [0.0, 1e-30, -1e-22, 1e-3, 1e2, 0.0, 1e-3, 1e-3, 1e2]
+    v0 = [0.0, 0.0, 0.0, 1e-30, 1e-12, 1.0, 1.0, 1e30, 3e38]
+    for n in (9, 9 * 40000):
+        m, v = (torch.tensor(a, device="cuda").repeat(n // 9) for a in (m0, v0))
+        x, g, t = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.full((), 9.0, device="cuda")
+        optim.adam_step([x], [g], [m], [v], [t], 0.5, (0.9, 0.99), eps)
+        d = np.sqrt(v.double().cpu().numpy()) / math.sqrt(1 - 0.99 ** 10) + eps
+        want = -0.5 / (1 - 0.9 ** 10) * m.double().cpu().numpy() / d
+        got = x.double().cpu().numpy()
+        big = np.abs(want) > 3.5e38
+        assert np.all(np.isinf(got[big]) & (np.sign(got[big]) == np.sign(want[big])))
+        err = np.abs(got[~big] - want[~big]) - (10 * 2.0 ** -24 * np.abs(want[~big]) + 2.0 ** -126)
+        assert np.all(err <= 0), (eps, n, got[:9], want[:9])
+
+
 def test_adam_keeps_infinite_parameters_apart_from_their_moments():
     torch, optim = _t()
     x, g = torch.full((5,), math.inf, device="cuda"), torch.ones(5, device="cuda")
