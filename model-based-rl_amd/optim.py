@@ -83,7 +83,7 @@ class FusedAdam(torch.optim.Optimizer):
     lr and weight_decay go by parameter group; betas, eps and decoupled_weight_decay are the same for all groups.  State is
     named and shaped as torch.optim.Adam's (float32 moments for 16-bit parameters), so a state_dict of either loads
     into the other.  The step counts live on the device: a captured step() counts on with every replay (with the learning
-    rates of its capture)."""
+    rates of its capture).  The first step of a parameter makes its state and cannot be captured."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False,
                  max_norm=None, norm_type=2.0):
@@ -131,6 +131,9 @@ class FusedAdam(torch.optim.Optimizer):
                     continue
                 s = state[p]
                 if "exp_avg" not in s:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("FusedAdam: take a first step before it is captured into a graph (a replay would zero "
+                                           "the state that it makes)")
                     self._new_state(p)
                 params.append(p)
                 grads.append(g)

@@ -638,6 +638,21 @@ def test_fused_adam_captured():
             assert float(opts[1].state[q]["step"]) == k + 2
 
 
+def test_fused_adam_refuses_a_first_step_under_capture():
+    """Its state would be zeroed by every replay."""
+    torch, optim = _t()
+    x = torch.ones(5, device="cuda", requires_grad=True)
+    x.grad = torch.ones_like(x)
+    opt = optim.FusedAdam([x], 0.01)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.zeros(1, device="cuda")
+        with pytest.raises(RuntimeError, match="before it is captured"):
+            opt.step()
+    assert bool((x == 1).all()) and not opt.state[x]
+    opt.step()
+    assert float(opt.state[x]["step"]) == 1.0
+
+
 def test_fused_adam_saves_and_goes_on():
     """16-bit parameters with their float32 moments, many of them: saved, loaded into a new optimiser, the same bits from there on.
     A closure, a scheduler, and a parameter of permuted dimensions on the way."""
