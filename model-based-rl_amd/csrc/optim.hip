@@ -46,6 +46,9 @@ constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 // launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.7 / 5.0 for 4.6 / 8.1, clipping of
 // 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 11e3 6.5 / 6.8 for 5.5 / 9.0.  Twice as much is slower both ways for the last two.
 constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;
+// And tensors, of which a wave takes 1 in 16 one after another: clipping of 64 (4000 values) 8.8 / 9.3 for 7.2 / 10.5, of 96 11.6 /
+// 12.1 for 7.3 / 11.3; the norm of 128 8.1 / 8.9 for 5.3 / 10.3, of 160 9.5 / 10.2 for 5.3 / 11.5.
+constexpr int kSmallNormCount = 128, kSmallClipCount = 64;
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
 constexpr int kSmallShift = 8;            // units of one 1 KB load a wave: 800-value tensors 6.6 us for 7.2 with twice that (Adam)
 
@@ -104,22 +107,84 @@ __device__ __forceinline__ void by_type(int code, F &&f) {
 }
 
 // ---- lists in kernel arguments ----
-template <int K_> struct Units {
+// A list of up to kFew tensors has a size of its own: filling 4 KB of arguments takes the host 0.5 us more than 350 bytes.  The
+// others hold as many as can be in the 4 KB of a launch, and are packed for it (device addresses have 48 bits): 400 tensors take
+// 2 launches for their sums and 4 for their update instead of 3 and 5 with fields of 8 bytes (8e6 float32 values: norm 14.3 us ->
+// 11.6, clipping 31.2 -> 25.2, Adam clipped 79 -> 73).  Unpacking is waited for where one block does it all: 16 tensors of
+// 500 values 5.65 us for 5.05 (Adam).
+constexpr int kFew = 16;
+__host__ __device__ __forceinline__ void *address(uint32_t lo, uint32_t hi) { return reinterpret_cast<void *>(uint64_t(hi) << 32 | lo); }
+__host__ __forceinline__ uint32_t upper(const void *p) { return uint32_t(uintptr_t(p) >> 32); }
+
+template <int K_, bool = (K_ > kFew)> struct Units {
     static constexpr int K = K_;
-    uint64_t n[K];        // values << 8 | head << 2 | type code
     uint32_t end[K];      // units of the tensors up to and including this one
+    uint32_t n[K];        // values, the lower 32 bits
+    uint32_t rest[K];     // the upper 6 | type code << 6 | head << 8; the upper half is the list's
     int count, shift;
     uint32_t units;
+    __device__ __forceinline__ int64_t values(int t) const { return int64_t(rest[t] & 63) << 32 | n[t]; }
+    __device__ __forceinline__ int type(int t) const { return rest[t] >> 6 & 3; }
+    __device__ __forceinline__ int head(int t) const { return rest[t] >> 8 & 63; }
+    void put(int t, int64_t values, int type, int64_t head) {
+        n[t] = uint32_t(values);
+        rest[t] = uint32_t(values >> 32) | uint32_t(type) << 6 | uint32_t(head) << 8;
+    }
 };
-template <int K> struct NormList { Units<K> u; void *x[K]; };
-template <int K> struct BeginList { Units<K> u; const void *x[K]; float *step[K]; double lr[K], wd[K]; };       // x: gradients
-template <int K> struct UpdateList { Units<K> u; const void *x[K]; void *p[K], *m[K], *v[K]; };
-template <int K> struct SmallList { UpdateList<K> l; float *step[K]; double lr[K], wd[K]; };                    // both, for one launch
+template <int K_> struct Units<K_, false> {
+    static constexpr int K = K_;
+    uint64_t n[K];        // values << 8 | head << 2 | type code
+    uint32_t end[K];
+    int count, shift;
+    uint32_t units;
+    __device__ __forceinline__ int64_t values(int t) const { return n[t] >> 8; }
+    __device__ __forceinline__ int type(int t) const { return n[t] & 3; }
+    __device__ __forceinline__ int head(int t) const { return n[t] >> 2 & 63; }
+    void put(int t, int64_t values, int type, int64_t head) { n[t] = uint64_t(values) << 8 | uint64_t(head) << 2 | uint64_t(type); }
+};
+// Lists of one tensor each (x), and of a gradient with its parameter, m and v; put() comes after the units' own.
+template <int K, bool = (K > kFew)> struct Ones {
+    Units<K> u;
+    uint32_t lo[K];
+    __device__ __forceinline__ void *x(int t) const { return address(lo[t], u.rest[t] >> 16); }
+    void put(int t, const void *p) {
+        lo[t] = uint32_t(uintptr_t(p));
+        u.rest[t] |= upper(p) << 16;
+    }
+};
+template <int K> struct Ones<K, false> {
+    Units<K, false> u;
+    const void *at[K];
+    __device__ __forceinline__ void *x(int t) const { return const_cast<void *>(at[t]); }
+    void put(int t, const void *p) { at[t] = p; }
+};
+template <int K, bool = (K > kFew)> struct Fours {
+    Units<K> u;
+    struct { uint32_t lo[4], hi[2]; } at[K];
+    template <int I> __device__ __forceinline__ void *get(int t) const { return address(at[t].lo[I], at[t].hi[I / 2] >> I % 2 * 16 & 0xffff); }
+    void put(int t, const void *g, const void *p, const void *m, const void *v) {
+        const void *a[4] = {g, p, m, v};
+        for (int i = 0; i < 4; i++) at[t].lo[i] = uint32_t(uintptr_t(a[i]));
+        for (int i = 0; i < 2; i++) at[t].hi[i] = upper(a[2 * i]) | upper(a[2 * i + 1]) << 16;
+    }
+    __device__ __forceinline__ void *x(int t) const { return get<0>(t); }
+};
+template <int K> struct Fours<K, false> {
+    Units<K, false> u;
+    const void *at[4][K];
+    template <int I> __device__ __forceinline__ void *get(int t) const { return const_cast<void *>(at[I][t]); }
+    void put(int t, const void *g, const void *p, const void *m, const void *v) { at[0][t] = g, at[1][t] = p, at[2][t] = m, at[3][t] = v; }
+    __device__ __forceinline__ void *x(int t) const { return get<0>(t); }
+};
+template <int K> using NormList = Ones<K>;
+template <int K> using UpdateList = Fours<K>;
+template <int K> using SmallNorm = Ones<K, false>;        // for one block
+template <int K> struct BeginList : Ones<K> { float *step[K]; double lr[K], wd[K]; };        // of the gradients
+template <int K> struct SmallAdam { Fours<K, false> l; float *step[K]; double lr[K], wd[K]; };          // both, for one block
 template <int K> struct CountList { float *step[K]; double lr[K], wd[K]; int count; };
-// How many fit 4 KB, and a size of its own for few: filling 4 KB of arguments takes the host 0.5 us more than 350 bytes.
-constexpr int kFew = 16, kNormList = 192, kAdamList = 80, kSmallList = 52, kCountList = 160;
-static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kAdamList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
-              sizeof(SmallList<kSmallList>) <= 3968 && sizeof(CountList<kCountList>) <= 3968, "kernel arguments are 4 KB");
+constexpr int kNormList = 246, kBeginList = 98, kAdamList = 109, kSmallAdamCount = 58, kCountList = 160;
+static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kBeginList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
+              sizeof(SmallAdam<kSmallAdamCount>) <= 3968 && sizeof(CountList<kCountList>) <= 3968, "kernel arguments are 4 KB");
 
 // What the update of one tensor multiplies with.
 struct Scalars { double size, root, keep, l2; };
@@ -150,13 +215,12 @@ template <class U>
 __device__ __forceinline__ Piece piece(const U &u, int t, uint32_t &unit, uint32_t stop) {
     Piece p;
     p.t = t;
-    const uint64_t n = u.n[t];
     const uint32_t end = min(stop, u.end[t]), skipped = unit - (t ? u.end[t - 1] : 0);
-    const int head = int(n >> 2 & 63);
-    p.type = int(n & 3);
+    const int head = u.head(t);
+    p.type = u.type(t);
     p.head = skipped ? 0 : head;
     p.first = head + (int64_t(skipped) << u.shift);
-    p.n = int(min(int64_t(n >> 8) - p.first, int64_t(end - unit) << u.shift));
+    p.n = int(min(u.values(t) - p.first, int64_t(end - unit) << u.shift));
     unit = end;
     return p;
 }
@@ -248,7 +312,7 @@ template <int P, bool kStream, class L>
 __device__ __forceinline__ double grid_norm(const L &l) {
     double acc = 0.0;
     walk<kStream>(l.u, [&](const Piece &p) {
-        by_type(p.type, [&](auto e) { acc = piece_norm<P, kStream>(e, l.x[p.t], p, acc); });
+        by_type(p.type, [&](auto e) { acc = piece_norm<P, kStream>(e, l.x(p.t), p, acc); });
     });
     return block_join<P, kWaves>(acc);
 }
@@ -256,7 +320,7 @@ template <int P, class L>
 __device__ __forceinline__ double small_norm(const L &l) {
     double acc = 0.0;
     shared_out(l.u, wave_of_block(), kSmallWaves, [&](const Piece &p) {
-        by_type(p.type, [&](auto e) { acc = piece_norm<P, false>(e, l.x[p.t], p, acc); });
+        by_type(p.type, [&](auto e) { acc = piece_norm<P, false>(e, l.x(p.t), p, acc); });
     });
     return block_join<P, kSmallWaves>(acc);
 }
@@ -351,7 +415,7 @@ __global__ __launch_bounds__(kThreads) void clip_scale(const L l, const double *
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = s;
     if (c == 1.0) return;
     walk<kStream>(l.u, [&](const Piece &p) {
-        by_type(p.type, [&](auto e) { piece_scale<kStream>(e, l.x[p.t], p, c); });
+        by_type(p.type, [&](auto e) { piece_scale<kStream>(e, l.x(p.t), p, c); });
     });
 }
 
@@ -364,7 +428,7 @@ __global__ __launch_bounds__(kSmallThreads) void norm_small(const L l, double ma
         const double c = factor_of(s, max_norm);
         if (c == 1.0) return;
         shared_out(l.u, wave_of_block(), kSmallWaves, [&](const Piece &p) {
-            by_type(p.type, [&](auto e) { piece_scale<false>(e, l.x[p.t], p, c); });
+            by_type(p.type, [&](auto e) { piece_scale<false>(e, l.x(p.t), p, c); });
         });
     }
 }
@@ -420,9 +484,9 @@ __device__ __forceinline__ void piece_adam(E, const L &l, const Piece &q, const 
     using T = typename E::T;
     using C = typename E::C;
     constexpr int V = sizeof(C) == 8 ? 2 : 4, kStep = kWave * V;
-    T *p = static_cast<T *>(l.p[q.t]) + q.first;
-    const T *g = static_cast<const T *>(l.x[q.t]) + q.first;
-    C *m = static_cast<C *>(l.m[q.t]) + q.first, *v = static_cast<C *>(l.v[q.t]) + q.first;
+    T *p = static_cast<T *>(l.template get<1>(q.t)) + q.first;
+    const T *g = static_cast<const T *>(l.x(q.t)) + q.first;
+    C *m = static_cast<C *>(l.template get<2>(q.t)) + q.first, *v = static_cast<C *>(l.template get<3>(q.t)) + q.first;
     const Update<C, kStream> f{C(b.b1), C(1.0 - b.b1), C(b.b2), C(1.0 - b.b2), C(b.eps), C(s.size), C(s.root), C(s.keep), C(s.l2), Factor<C>(clip)};
     const int lane = threadIdx.x % kWave, n = q.n;
     auto some = [&](int i, auto count) {        // `count` vectors a lane, all on their way at once
@@ -475,8 +539,10 @@ __global__ __launch_bounds__(kCountList) void adam_count(const CountList<kCountL
     if (i < l.count) scalars[i] = count_step(l.step[i], l.lr[i], l.wd[i], b, decoupled);
 }
 
+// Streaming: 7 waves a SIMD, by the compiler's own choice or not (kAdamShift; two registers too many leave 6: bfloat16, 268e6 values
+// clipped: 1.03 ms for 1.01).
 template <int P, bool kStream, class L>
-__global__ __launch_bounds__(kThreads) void adam_update(const L l, const Betas b, const Scalars *scalars, const double *part, int parts,
+__global__ __launch_bounds__(kThreads, kStream ? 7 : 1) void adam_update(const L l, const Betas b, const Scalars *scalars, const double *part, int parts,
                                                         double max_norm, double *norm) {
     double clip = 1.0;
     if constexpr (P != kNoClip) {
@@ -544,8 +610,8 @@ void fill_list(List &l, int64_t from, int64_t to, const int64_t *numel, const in
         const int at = int(i - from);
         const int64_t h = std::min<int64_t>(numel[i], head(i));
         if (numel[i]) units += uint32_t(std::max<int64_t>((numel[i] - h + (int64_t(1) << shift) - 1) >> shift, 1));
-        l.u.n[at] = uint64_t(numel[i]) << 8 | uint64_t(h) << 2 | uint64_t(dtype[i]);
         l.u.end[at] = units;
+        l.u.put(at, numel[i], dtype[i], h);
         fill(at, i);
     }
     l.u.count = int(to - from);
@@ -588,6 +654,9 @@ int check_list(const char *what, int64_t count, const int64_t *numel, const int 
     return 0;
 }
 
+// Whether a list can hold the address of a tensor with values.
+bool usable(const void *p) { return p && !(uintptr_t(p) >> 48); }
+
 // Memory that is written must not be any other memory of the call.
 struct Ranges {
     struct Range { uintptr_t lo, hi; bool written; };
@@ -628,8 +697,9 @@ int launched(const char *what) {
 
 // Whether one block takes a list on alone.
 bool small(int op, int64_t count, const int64_t *numel, const int *dtype) {
-    if (op == MBRL_OP_ADAM) return count <= kSmallList && adam_bytes(count, numel, dtype) <= kSmallAdam;
-    return count <= kNormList && total_bytes(count, numel, dtype) <= (op == MBRL_OP_CLIP ? kSmallClip : kSmallNorm);
+    if (op == MBRL_OP_ADAM) return count <= kSmallAdamCount && adam_bytes(count, numel, dtype) <= kSmallAdam;
+    const bool clip = op == MBRL_OP_CLIP;
+    return count <= (clip ? kSmallClipCount : kSmallNormCount) && total_bytes(count, numel, dtype) <= (clip ? kSmallClip : kSmallNorm);
 }
 
 // Workspace of the others: [total, unused][partial sums][Scalars of each tensor]
@@ -660,7 +730,7 @@ struct Gradients {
         constexpr int K = decltype(l.u)::K;
         l.u.count = l.u.units = 0;
         for (int64_t i = 0; i < count; i += K) {
-            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head, [&](int at, int64_t k) { l.x[at] = x[k]; });
+            fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head, [&](int at, int64_t k) { l.put(at, x[k]); });
             go();
         }
     }
@@ -696,10 +766,10 @@ struct Runs : Gradients {
 
 // Calls f(the flag as a constant).
 template <class F> void by_flag(bool flag, F &&f) { flag ? f(std::true_type{}) : f(std::false_type{}); }
-// Calls f(a list of the smallest size): few tensors have one of their own, but where memory is what counts.
+// Calls f(a list of the smallest size).
 template <template <int> class List, int K, class F>
-void by_count(int64_t count, bool stream, F &&f) {
-    if (count <= kFew && !stream) f(List<kFew>{});
+void by_count(int64_t count, F &&f) {
+    if (count <= kFew) f(List<kFew>{});
     else f(List<K>{});
 }
 
@@ -719,7 +789,7 @@ Parts launch_partials(const Gradients &g, bool stream, bool finish, const Space 
     int parts = 0;
     by_flag(stream, [&](auto stream_) {
         constexpr bool kStream = stream_;
-        by_count<NormList, kNormList>(g.count, kStream, [&](auto l) {
+        by_count<NormList, kNormList>(g.count, [&](auto l) {
             g.lists(l, unit_shift(g.values), from_first, [&] {
                 if (const int grid = grid_of(l.u, kMaxBlocks, kStream ? 1 : kUnits)) {
                     hipLaunchKernelGGL((norm_partials<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, ws.part + parts);
@@ -738,7 +808,7 @@ void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm,
         constexpr int P = P_;
         if constexpr (P != kNoClip) {
             if (small(kClip ? MBRL_OP_CLIP : MBRL_OP_NORM, g.count, g.numel, g.dtype)) {
-                by_count<NormList, kNormList>(g.count, false, [&](auto l) {
+                by_count<SmallNorm, kSmallNormCount>(g.count, [&](auto l) {
                     g.lists(l, kSmallShift, from_first, [] {});
                     hipLaunchKernelGGL((norm_small<P, kClip, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, max_norm, norm);
                 });
@@ -751,7 +821,7 @@ void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm,
                 auto head = [&](int64_t i) { return before_line(runs.x[i], kSize[runs.dtype[i]]); };
                 by_flag(stream, [&](auto stream_) {
                     constexpr bool kStream = stream_;
-                    by_count<NormList, kNormList>(runs.count, kStream, [&](auto l) {
+                    by_count<NormList, kNormList>(runs.count, [&](auto l) {
                         runs.lists(l, !kStream ? unit_shift(g.values) : g.bytes == 2 * g.values ? kScaleShift16 : kScaleShift, head, [&] {
                             if (const int grid = grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks, kUnits))
                                 hipLaunchKernelGGL((clip_scale<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, sum.part, sum.parts,
@@ -793,7 +863,7 @@ int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel
         if (!norm || (need && !workspace) || (count && !grads)) return report(-1, "mbrl_grad_norm: null argument");
         if (workspace_bytes < need) return report(-8, "mbrl_grad_norm: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
-            if (numel[i] && !grads[i]) return report(-1, "mbrl_grad_norm: null tensor");
+            if (numel[i] && !usable(grads[i])) return report(-1, "mbrl_grad_norm: null tensor, or no device address");
         launch_norm<false>(norm_type, Gradients(count, const_cast<void *const *>(grads), numel, dtype), Space(workspace, count), 0.0, norm,
                            (hipStream_t)hip_stream);
         return launched("mbrl_grad_norm");
@@ -812,7 +882,7 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
         Ranges r;
         r.r.reserve(count);
         for (int64_t i = 0; i < count; i++) {
-            if (numel[i] && !grads[i]) return report(-1, "mbrl_clip_grad_norm: null tensor");
+            if (numel[i] && !usable(grads[i])) return report(-1, "mbrl_clip_grad_norm: null tensor, or no device address");
             r.add(grads[i], numel[i] * kSize[dtype[i]], true);
         }
         if (!r.disjoint()) return report(-7, "mbrl_clip_grad_norm: two of the tensors share memory");
@@ -837,8 +907,8 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             return report(-1, "mbrl_adam_step: null argument");
         if (workspace_bytes < need) return report(-8, "mbrl_adam_step: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
-            if (!steps[i] || (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i])))
-                return report(-1, "mbrl_adam_step: null tensor");
+            if (!steps[i] || (numel[i] && !(usable(params[i]) && usable(grads[i]) && usable(exp_avgs[i]) && usable(exp_avg_sqs[i]))))
+                return report(-1, "mbrl_adam_step: null tensor, or no device address");
         Ranges r;
         r.r.reserve(5 * count);
         auto add = [&](auto x, bool written, auto bytes) {
@@ -862,18 +932,17 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             constexpr int K = std::decay_t<decltype(l.u)>::K;
             l.u.count = l.u.units = 0;
             for (int64_t i = 0; i < count; i += K) {
-                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head,
-                          [&](int at, int64_t k) { l.x[at] = grads[k]; fill(at, k); });
+                fill_list(l, i, std::min<int64_t>(count, i + K), numel, dtype, shift, head, fill);
                 go(i);
             }
         };
-        auto tensors = [&](auto &l) { return [&](int at, int64_t k) { l.p[at] = params[k]; l.m[at] = exp_avgs[k]; l.v[at] = exp_avg_sqs[k]; }; };
+        auto tensors = [&](auto &l) { return [&](int at, int64_t k) { l.put(at, grads[k], params[k], exp_avgs[k], exp_avg_sqs[k]); }; };
         auto counters = [&](auto &l) { return [&](int at, int64_t k) { l.step[at] = steps[k]; l.lr[at] = lr[k]; l.wd[at] = weight_decay[k]; }; };
         by_norm(clip ? norm_type : kNoClip, [&](auto P_) {
             constexpr int P = P_;
             constexpr bool kClip = P != kNoClip;
             if (small(MBRL_OP_ADAM, count, numel, dtype)) {
-                by_count<SmallList, kSmallList>(count, false, [&](auto l) {
+                by_count<SmallAdam, kSmallAdamCount>(count, [&](auto l) {
                     lists(l.l, kSmallShift, from_first, [&](int at, int64_t k) { tensors(l.l)(at, k); counters(l)(at, k); }, [](int64_t) {});
                     hipLaunchKernelGGL((adam_small<P, decltype(l)>), dim3(1), dim3(kSmallThreads), 0, st, l, b, decoupled, max_norm, norm);
                 });
@@ -883,11 +952,11 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             const int shift = unit_shift(values);
             auto head = [&](int64_t i) { return before_line(exp_avgs[i], kSize[dtype[i]] == 8 ? 8 : 4); };
             Parts sum{nullptr, 0};
-            if (count <= kAdamList) {
+            if (count <= kBeginList) {
                 by_flag(kClip && total_bytes(count, numel, dtype) > kCache, [&](auto stream_) {
                     constexpr bool kStream = kClip && stream_;
-                    by_count<BeginList, kAdamList>(count, kStream, [&](auto l) {
-                        lists(l, shift, from_first, counters(l), [&](int64_t) {
+                    by_count<BeginList, kBeginList>(count, [&](auto l) {
+                        lists(l, shift, from_first, [&](int at, int64_t k) { l.put(at, grads[k]); counters(l)(at, k); }, [&](int64_t) {
                             const int grid = kClip ? std::max(grid_of(l.u), 1) : 1;
                             hipLaunchKernelGGL((adam_begin<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, decoupled,
                                                ws.scalars, ws.part);
@@ -909,7 +978,7 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             }
             by_flag(stream, [&](auto stream_) {
                 constexpr bool kStream = stream_;
-                by_count<UpdateList, kAdamList>(count, kStream, [&](auto l) {
+                by_count<UpdateList, kAdamList>(count, [&](auto l) {
                     lists(l, !kStream ? shift : bytes == 32 * values ? kAdamShift64 : kAdamShift, head, tensors(l), [&](int64_t i) {
                         if (const int grid = std::max(grid_of(l.u, kStream ? kStreamBlocks : kMaxBlocks), kClip && i == 0 ? 1 : 0))        // one block at least writes the norm
                             hipLaunchKernelGGL((adam_update<P, kStream, decltype(l)>), dim3(grid), dim3(kThreads), 0, st, l, b, ws.scalars + i,

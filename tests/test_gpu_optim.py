@@ -123,6 +123,20 @@ def test_many_tensors(count):
     check_adam(sizes, ["float32", "bfloat16"], most=0.5, misaligned=True)
 
 
+@pytest.mark.parametrize("count", [16, 17, 58, 59, 98, 99, 109, 110, 128, 129, 160, 161, 246, 247, 492, 493])
+def test_list_borders(count):
+    """Around the sizes of lists and the numbers of tensors that one block takes on: lists of short tensors, and of one long one
+    among them, which need not be short."""
+    rng = np.random.default_rng(count)
+    sizes = [(int(rng.integers(1, 60)),) for _ in range(count)]
+    check_clip(sizes, TYPES, 0.4, misaligned=True)
+    check_adam(sizes, TYPES, most=0.5, misaligned=True, steps=1)
+    sizes[count // 2] = (70001,)
+    check_clip(sizes, ["float32", "float16"], 0.4)
+    check_adam(sizes, ["float32", "float16"], steps=1)
+    check_adam(sizes, ["bfloat16", "float64"], most=0.5, steps=1)
+
+
 def test_empty_lists_and_zeros():
     torch, optim = _t()
     for ts in ([], [torch.zeros(0, device="cuda")], [torch.zeros((0, 4), device="cuda", dtype=torch.float16)] * 3):
@@ -578,6 +592,20 @@ def test_more_values_than_32_bits_count():
     assert float(optim.grad_norm([x])) == math.sqrt(45.0)
     optim.clip_grad_norm_([x], 0.5 * (math.sqrt(45.0) + 1e-6))
     assert x[at].tolist() == [1.5] * 5 and int(torch.count_nonzero(x)) == 5
+
+
+@pytest.mark.parametrize("others", [0, 16, 300])
+def test_more_values_than_fit_32_bits(others):
+    """2^32 + 4099 float16 values (8 GiB), alone and among short tensors: the last ones count, and are reached."""
+    torch, optim = _t()
+    n = (1 << 32) + 4099
+    x = torch.zeros(n, dtype=torch.float16, device="cuda")
+    x[0], x[-1], x[-4099] = 3.0, 4.0, 12.0
+    ts = [torch.zeros(5, device="cuda") for _ in range(others)]
+    ts.insert(others // 2, x)
+    assert float(optim.grad_norm(ts)) == 13.0 and float(optim.grad_norm(ts, math.inf)) == 12.0
+    assert float(optim.clip_grad_norm_(ts, 6.5)) == 13.0
+    assert [float(x[i]) for i in (0, -1, -4099)] == [1.5, 2.0, 6.0] and int((x != 0).sum(dtype=torch.int64)) == 3
 
 
 def test_a_run_of_them_together():

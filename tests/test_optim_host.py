@@ -137,6 +137,20 @@ def test_abi_refusals():
     assert L.mbrl_grad_norm(*good, 5, ws, big, norm, None) == -7
 
 
+def test_abi_refuses_what_is_no_device_address():
+    L = lib.load()
+    ws, norm, at = C.c_void_p(0x1000), C.c_void_p(0x8000), 1 << 48
+    l = _arrays([0x10000, at], [16, 16], [1, 1])
+    assert L.mbrl_grad_norm(*l, 2, ws, 1 << 20, norm, None) == -1 and b"address" in L.mbrl_last_error()
+    assert L.mbrl_clip_grad_norm(*l, 2, 1.0, ws, 1 << 20, norm, None) == -1
+    good = [0x10000, 0x20000, 0x30000, 0x40000]
+    f64, step = (C.c_double * 1)(0.0), (C.c_void_p * 1)(0x50000)
+    for i in range(4):
+        ptrs = [(C.c_void_p * 1)(at if k == i else p) for k, p in enumerate(good)]
+        assert L.mbrl_adam_step(1, *ptrs, step, (C.c_int64 * 1)(16), (C.c_int * 1)(1), f64, f64, 0.9, 0.999, 1e-8, 0, 2, 1.0, ws, 1 << 20,
+                                None, None) == -1 and b"address" in L.mbrl_last_error()
+
+
 def test_fused_adam_construction_and_state_dict():
     p = [torch.nn.Parameter(Z(3)), torch.nn.Parameter(Z(2, 2, dtype=torch.bfloat16))]
     for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(max_norm=-1.0), dict(norm_type=3)):
