@@ -181,10 +181,29 @@ template <int K> using UpdateList = Fours<K>;
 template <int K> using SmallNorm = Ones<K, false>;        // for one block
 template <int K> struct BeginList : Ones<K> { float *step[K]; double lr[K], wd[K]; };        // of the gradients
 template <int K> struct SmallAdam { Fours<K, false> l; float *step[K]; double lr[K], wd[K]; };          // both, for one block
-template <int K> struct CountList { float *step[K]; double lr[K], wd[K]; int count; };
-constexpr int kNormList = 246, kBeginList = 98, kAdamList = 109, kSmallAdamCount = 58, kCountList = 160;
+// Steps alone.  Their rates come from few groups: the list holds each pair once.
+constexpr int kCountList = 416, kRates = 64;
+struct CountList {
+    double lr[kRates], wd[kRates];
+    uint32_t lo[kCountList];
+    uint16_t hi[kCountList];
+    uint8_t rate[kCountList];
+    int count, rates;
+    // false: full
+    bool put(float *step, double lr_, double wd_) {
+        int k = 0;
+        while (k < rates && !(lr[k] == lr_ && wd[k] == wd_)) k++;
+        if (count == kCountList || k == kRates) return false;
+        if (k == rates) lr[k] = lr_, wd[k] = wd_, rates++;
+        lo[count] = uint32_t(uintptr_t(step));
+        hi[count] = uint16_t(upper(step));
+        rate[count++] = uint8_t(k);
+        return true;
+    }
+};
+constexpr int kNormList = 246, kBeginList = 98, kAdamList = 109, kSmallAdamCount = 58;
 static_assert(sizeof(NormList<kNormList>) <= 3968 && sizeof(BeginList<kBeginList>) <= 3968 && sizeof(UpdateList<kAdamList>) <= 3968 &&
-              sizeof(SmallAdam<kSmallAdamCount>) <= 3968 && sizeof(CountList<kCountList>) <= 3968, "kernel arguments are 4 KB");
+              sizeof(SmallAdam<kSmallAdamCount>) <= 3968 && sizeof(CountList) <= 3968, "kernel arguments are 4 KB");
 
 // What the update of one tensor multiplies with.
 struct Scalars { double size, root, keep, l2; };
@@ -534,9 +553,11 @@ __global__ __launch_bounds__(kThreads) void adam_begin(const L l, const Betas b,
 }
 
 // For lists too long for that: the steps apart, the norm as of any list.
-__global__ __launch_bounds__(kCountList) void adam_count(const CountList<kCountList> l, const Betas b, int decoupled, Scalars *scalars) {
-    const int i = threadIdx.x;
-    if (i < l.count) scalars[i] = count_step(l.step[i], l.lr[i], l.wd[i], b, decoupled);
+__global__ __launch_bounds__(kThreads) void adam_count(const CountList l, const Betas b, int decoupled, Scalars *scalars) {
+    const int i = blockIdx.x * kThreads + threadIdx.x;
+    if (i >= l.count) return;
+    const int k = l.rate[i];
+    scalars[i] = count_step(static_cast<float *>(address(l.lo[i], l.hi[i])), l.lr[k], l.wd[k], b, decoupled);
 }
 
 // Streaming: 7 waves a SIMD, by the compiler's own choice or not (kAdamShift; two registers too many leave 6: bfloat16, 268e6 values
@@ -661,14 +682,12 @@ bool usable(const void *p) { return p && !(uintptr_t(p) >> 48); }
 struct Ranges {
     struct Range { uintptr_t lo, hi; bool written; };
     std::vector<Range> r;
+    std::vector<size_t> lists;        // where each list ends
     void add(const void *p, int64_t bytes, bool written) {
         if (bytes) r.push_back({uintptr_t(p), uintptr_t(p) + uintptr_t(bytes), written});
     }
+    void close() { lists.push_back(r.size()); }
     bool disjoint() const {
-        // Device addresses have 48 bits: with the place behind them they are sorted as plain numbers, four times as fast
-        // as the ranges themselves (900 of them: 8 us for 34), which a long list's step would wait for.
-        std::vector<uint64_t> order;
-        order.reserve(r.size());
         uintptr_t read_end = 0, write_end = 0;
         auto next = [&](const Range &x) {
             if (x.lo < write_end || (x.written && x.lo < read_end)) return false;
@@ -676,11 +695,22 @@ struct Ranges {
             end = std::max(end, x.hi);
             return true;
         };
-        bool packed = r.size() <= 0x10000;
-        for (const Range &x : r) packed = packed && x.lo < (uintptr_t(1) << 48);
-        for (size_t i = 0; i < r.size(); i++) order.push_back(packed ? uint64_t(r[i].lo) << 16 | i : i);
-        if (packed) std::sort(order.begin(), order.end());
-        else std::sort(order.begin(), order.end(), [&](uint64_t a, uint64_t b) { return r[a].lo < r[b].lo; });
+        // Addresses have 48 bits: with the place behind them they are sorted as plain numbers, four times as fast as the ranges
+        // themselves.  Lists mostly lie in order, or nearly so, and are only merged then (402 tensors and their four others: 1
+        // to 5 us for 14 to 20, which a step would wait for).
+        std::vector<uint64_t> order(r.size());
+        const bool packed = r.size() <= 0x10000;
+        for (size_t i = 0; i < r.size(); i++) order[i] = packed ? uint64_t(r[i].lo) << 16 | i : i;
+        const auto begin = order.begin();
+        if (packed) {
+            size_t from = 0;
+            for (size_t to : lists) {
+                if (!std::is_sorted(begin + from, begin + to)) std::sort(begin + from, begin + to);
+                if (from && from < to && order[from] < order[from - 1]) std::inplace_merge(begin, begin + from, begin + to);
+                from = to;
+            }
+        } else
+            std::sort(begin, order.end(), [&](uint64_t a, uint64_t b) { return r[a].lo < r[b].lo; });
         for (uint64_t i : order)
             if (!next(r[packed ? i & 0xffff : i])) return false;
         return true;
@@ -885,6 +915,7 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
             if (numel[i] && !usable(grads[i])) return report(-1, "mbrl_clip_grad_norm: null tensor, or no device address");
             r.add(grads[i], numel[i] * kSize[dtype[i]], true);
         }
+        r.close();
         if (!r.disjoint()) return report(-7, "mbrl_clip_grad_norm: two of the tensors share memory");
         launch_norm<true>(norm_type, Gradients(count, grads, numel, dtype), Space(workspace, count), max_norm, norm, (hipStream_t)hip_stream);
         return launched("mbrl_clip_grad_norm");
@@ -907,12 +938,13 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
             return report(-1, "mbrl_adam_step: null argument");
         if (workspace_bytes < need) return report(-8, "mbrl_adam_step: workspace too small (mbrl_optim_workspace_bytes)");
         for (int64_t i = 0; i < count; i++)
-            if (!steps[i] || (numel[i] && !(usable(params[i]) && usable(grads[i]) && usable(exp_avgs[i]) && usable(exp_avg_sqs[i]))))
+            if (!usable(steps[i]) || (numel[i] && !(usable(params[i]) && usable(grads[i]) && usable(exp_avgs[i]) && usable(exp_avg_sqs[i]))))
                 return report(-1, "mbrl_adam_step: null tensor, or no device address");
         Ranges r;
         r.r.reserve(5 * count);
         auto add = [&](auto x, bool written, auto bytes) {
             for (int64_t i = 0; i < count; i++) r.add(x[i], bytes(i), written);
+            r.close();
         };
         auto own = [&](int64_t i) { return numel[i] * kSize[dtype[i]]; };
         auto wide = [&](int64_t i) { return numel[i] * (kSize[dtype[i]] == 8 ? 8 : 4); };
@@ -965,11 +997,11 @@ int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads,
                     });
                 });
             } else {
-                CountList<kCountList> l;
-                for (int64_t i = 0; i < count; i += kCountList) {
-                    l.count = int(std::min<int64_t>(count - i, kCountList));
-                    for (int k = 0; k < l.count; k++) counters(l)(k, i + k);
-                    hipLaunchKernelGGL(adam_count, dim3(1), dim3(kCountList), 0, st, l, b, decoupled, ws.scalars + i);
+                CountList l;
+                for (int64_t i = 0, from = 0; from < count; from = i) {
+                    l.count = l.rates = 0;
+                    while (i < count && l.put(steps[i], lr[i], weight_decay[i])) i++;
+                    hipLaunchKernelGGL(adam_count, dim3((l.count + kThreads - 1) / kThreads), dim3(kThreads), 0, st, l, b, decoupled, ws.scalars + from);
                 }
                 if constexpr (kClip) {
                     const Gradients g(count, const_cast<void *const *>(grads), numel, dtype);

@@ -325,6 +325,12 @@ def test_adam_of_one_tensor(n, dtype):
     check_adam([(n,)], [dtype], 0.5)
 
 
+@pytest.mark.parametrize("count,rates", [(99, 1), (99, 99), (130, 64), (130, 65), (416, 3), (417, 3), (600, 200)])
+def test_adam_rates_of_long_lists(count, rates):
+    """Learning rates of their own, more than a launch that counts the steps holds, and as many tensors."""
+    check_adam([(1 + 37 * i % 50,) for i in range(count)], ["float32"], wd=0.1, lrs=[1e-3 * (k + 1) / rates for k in range(rates)])
+
+
 def test_adam_of_the_smallest_and_largest_moments():
     """Second moments from nothing and subnormal values to the largest, with and without eps, against float64.  m, v, root, scale,
     sum, quotient, size and product: 12 half steps at most."""
