@@ -18,10 +18,10 @@
 // instructions (a division and a root among them) for the update.  Measured on an MI355X, where a copy of 4 GiB runs at 4.8
 // TB/s and x *= c at 5.9, 10 float32 tensors of as many values in all, every launch included:
 //   values    norm               clip (scaled)       Adam                Adam, clipped
-//   8e3       3.5 us             5.1 us              6.2 us              8.1 us         one launch
-//   5e5       4.9 us             6.7 us              6.1 us              7.9 us         two launches
+//   8e3       3.5 us             5.1 us              5.1 us              7.2 us         one launch
+//   5e5       4.8 us             6.7 us              5.8 us              7.7 us         two launches
 //   8e6       6.6 us, 4.9 TB/s   14.7 us, 6.5 TB/s   39 us, 5.7 TB/s     46 us          from the cache
-//   268e6     164 us, 6.5 TB/s   525 us, 6.1 TB/s    1.23 ms, 6.1 TB/s   1.40 ms        from memory
+//   268e6     164 us, 6.5 TB/s   525 us, 6.1 TB/s    1.22 ms, 6.2 TB/s   1.37 ms        from memory
 // (clip: two reads and a write).  Below that it is the launches: an empty one takes 2.2 us of the device and 3.7 us of the
 // host, so small lists are done in one (a call of 2 or 10 tensors: 4.3 us of the host for a norm).
 #include <hip/hip_runtime.h>
@@ -44,7 +44,8 @@ constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 
 // Bytes that one block of 16 waves takes on alone, in one launch (of gradients; of all four tensors for Adam).  Against the two
 // launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.7 / 5.0 for 4.6 / 8.1, clipping of
-// 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 11e3 6.5 / 6.8 for 5.5 / 9.0.  Twice as much is slower both ways for the last two.
+// 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 11e3 5.6 / 6.1 for 5.0 / 8.9 and clipped 7.8 / 8.1 for 6.9 / 9.8.  Twice as much is slower
+// both ways for the last two (24e3: 9.0 / 9.5 for 5.0 / 9.0, clipped 11.6 / 12.0 for 6.9 / 9.8).
 constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;
 // And tensors, of which a wave takes 1 in 16 one after another: clipping of 64 (4000 values) 8.8 / 9.3 for 7.2 / 10.5, of 96 11.6 /
 // 12.1 for 7.3 / 11.3; the norm of 128 8.1 / 8.9 for 5.3 / 10.3, of 160 9.5 / 10.2 for 5.3 / 11.5.
