@@ -64,8 +64,10 @@ constexpr int kMaxParts = 2048;           // partial sums that every block of a 
 // the update take short units in blocks that do not stay, so that what is under way at a time lies together.  268e6 float32
 // values: norm 161 us for 180, scaling 357 for 440, Adam 1226 for 1505.  From a quarter of the cache on it pays for data that
 // was not in it (float32, other tensors used between: clipping of 32e6 values 67 us for 81, Adam of 8e6 43 for 51; of 4e6 26
-// for 28) and costs little for data that was (65 -> 71, 38 -> 41).  A norm alone gains from half of it on (32e6: 25.2 us for
-// 27.1; 16e6: 17.3 for 17.0); before a scaling it leaves what it reads in the cache, up to its size (64e6: 126 us for 131).
+// for 28) and costs little for data that was (65 -> 71, 38 -> 41).  Sums gain from half of it on (a norm
+// of 32e6: 25.2 us for 27.1; 16e6: 17.3 for 17.0), before a scaling too, though it finds less in the cache then, if there is one:
+// 50e6 values 39.5 us for 42.8 untouched and 105 for 100 scaled, 117e6 of bfloat16 44 for 48.5 and 119 for 116.  Before an
+// update, which reads the gradients in any case, what is read stays in the cache, up to its size (50e6: 244 us for 258).
 constexpr int64_t kCache = int64_t(256) << 20;
 // Values of a unit.  Of the update one load a lane and tensor (268e6 float32 values: 1.23 ms for 1.30 with two, bfloat16 0.93 for
 // 1.04; 128e6 of float64, half as many a load: 1.19 for 1.25), compiled for that alone: 72 registers for 117 leave room for 7
@@ -846,7 +848,7 @@ void launch_norm(int kind, const Gradients &g, const Space &ws, double max_norm,
                 return;
             }
             const bool stream = g.bytes > kCache / 4;
-            const Parts sum = launch_partials<P>(g, g.bytes > (kClip ? kCache : kCache / 2), !kClip || stream, ws, norm, st);
+            const Parts sum = launch_partials<P>(g, g.bytes > kCache / 2, !kClip || stream, ws, norm, st);
             if constexpr (kClip) {
                 const Runs runs(g);
                 auto head = [&](int64_t i) { return before_line(runs.x[i], kSize[runs.dtype[i]]); };
