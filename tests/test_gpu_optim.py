@@ -461,6 +461,37 @@ def test_captured_and_replayed():
         optim.grad_norm(eager[1])
 
 
+@pytest.mark.parametrize("sizes", [[(40,), (6, 7)], [(1 + 37 * i % 90,) for i in range(450)], [(17_000_001,), (33,)]])
+def test_captured_and_replayed_lists_of_all_lengths(sizes):
+    """One block's work, several launches of counts, sums and updates, and lists beyond the cache: every replay gives the bits of
+    the eager calls."""
+    torch, optim = _t()
+    types = ["float32", "bfloat16"]
+
+    def state():
+        xs, gs = make(sizes, types, 35), make(sizes, types, 36)
+        ms, vs = ([torch.zeros(x.shape, device="cuda") for x in xs] for _ in range(2))
+        return xs, gs, ms, vs, [torch.zeros((), device="cuda") for _ in xs]
+
+    def one(s):
+        n = optim.clip_grad_norm_(s[1], 5.0)
+        return n, optim.adam_step(*s, [1e-3 * (1 + i % 70) for i in range(len(sizes))], max_norm=2.0)
+    eager, graphed, graph = state(), state(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norms = one(graphed)
+    for k in range(3):
+        for l in (eager, graphed):
+            for a, b in zip(l[1], make(sizes, types, 60 + k)):
+                a.copy_(b)
+        want = one(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert [float(a) for a in norms] == [float(a) for a in want]
+        for la, lb in zip(graphed, eager):
+            assert all(torch.equal(a, b) for a, b in zip(la, lb)), k
+        assert all(float(c) == k + 1 for c in graphed[4][:2])
+
+
 def test_streams_beside_each_other():
     torch, optim = _t()
     lists = [make([(200003,), (77,)], ["float32"], 60 + i) for i in range(4)]
