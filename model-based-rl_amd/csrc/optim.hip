@@ -18,9 +18,9 @@
 // instructions (a division and a root among them) for the update.  Measured on an MI355X, where a copy of 4 GiB runs at 4.8
 // TB/s and x *= c at 5.9, 10 float32 tensors of as many values in all, every launch included:
 //   values    norm               clip (scaled)       Adam                Adam, clipped
-//   8e3       3.5 us             5.1 us              5.1 us              7.2 us         one launch
-//   5e5       4.8 us             6.7 us              5.8 us              7.7 us         two launches
-//   8e6       6.6 us, 4.9 TB/s   14.7 us, 6.5 TB/s   39 us, 5.7 TB/s     46 us          from the cache
+//   8e3       3.5 us             5.1 us              6.2 us              8.3 us         one launch
+//   5e5       4.8 us             6.7 us              6.2 us              8.1 us         two launches
+//   8e6       6.6 us, 4.9 TB/s   14.7 us, 6.5 TB/s   40 us, 5.6 TB/s     46 us          from the cache
 //   268e6     164 us, 6.5 TB/s   525 us, 6.1 TB/s    1.22 ms, 6.2 TB/s   1.37 ms        from memory
 // (clip: two reads and a write).  Below that it is the launches: an empty one takes 2.2 us of the device and 3.7 us of the
 // host, so small lists are done in one (a call of 2 or 10 tensors: 4.3 us of the host for a norm).
@@ -44,14 +44,15 @@ constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 
 // Bytes that one block of 16 waves takes on alone, in one launch (of gradients; of all four tensors for Adam).  Against the two
 // launches of longer lists, device / host time in us for float32: norm of 64e3 values 4.7 / 5.0 for 4.6 / 8.1, clipping of
-// 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 11e3 5.6 / 6.1 for 5.0 / 8.9 and clipped 7.8 / 8.1 for 6.9 / 9.8.  Twice as much is slower
-// both ways for the last two (24e3: 9.0 / 9.5 for 5.0 / 9.0, clipped 11.6 / 12.0 for 6.9 / 9.8).
+// 24e3 6.7 / 6.9 for 6.0 / 8.7, Adam of 12e3 6.5 / 6.9 for 5.1 / 8.7 and clipped 8.8 / 9.2 for 7.0 / 9.6.  Twice as much is slower
+// both ways for the last two (24e3: 10.8 / 11.2 for 5.5 / 8.8, clipped 13.5 / 13.9 for 7.4 / 9.8).  The bounds go by the host's time,
+// that of a call; a replayed graph pays the device's alone, and would be better off with two launches near them.
 constexpr int64_t kSmallNorm = 256 << 10, kSmallClip = 96 << 10, kSmallAdam = 192 << 10;
 // And tensors, of which a wave takes 1 in 16 one after another: clipping of 64 (4000 values) 8.8 / 9.3 for 7.2 / 10.5, of 96 11.6 /
 // 12.1 for 7.3 / 11.3; the norm of 128 8.1 / 8.9 for 5.3 / 10.3, of 160 9.5 / 10.2 for 5.3 / 11.5.
 constexpr int kSmallNormCount = 128, kSmallClipCount = 64;
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
-constexpr int kSmallShift = 8;            // units of one 1 KB load a wave: 800-value tensors 6.6 us for 7.2 with twice that (Adam)
+constexpr int kSmallShift = 8;            // units of one 1 KB load a wave: 800-value tensors 6.2 us for 6.7 with twice that (Adam)
 
 // Middle lists: up to kMaxBlocks blocks (4 a CU) stay and take units of 2^9 values or more.  Clipping and norm walk a wave's units
 // one after another (walk()): 8e6 values 7.0 us for 10.2 dealt out in turn, 16e6 13.4 for 15.4.  Two units a wave at least:
@@ -114,7 +115,7 @@ __device__ __forceinline__ void by_type(int code, F &&f) {
 // others hold as many as can be in the 4 KB of a launch, and are packed for it (device addresses have 48 bits): 400 tensors take
 // 2 launches for their sums and 4 for their update instead of 3 and 5 with fields of 8 bytes (8e6 float32 values: norm 14.3 us ->
 // 11.6, clipping 31.2 -> 25.2, Adam clipped 79 -> 73).  Unpacking is waited for where one block does it all: 16 tensors of
-// 500 values 5.65 us for 5.05 (Adam).
+// 500 values 5.65 us for 5.05 (Adam, with the hardware's root and quotient).
 constexpr int kFew = 16;
 __host__ __device__ __forceinline__ void *address(uint32_t lo, uint32_t hi) { return reinterpret_cast<void *>(uint64_t(hi) << 32 | lo); }
 __host__ __forceinline__ uint32_t upper(const void *p) { return uint32_t(uintptr_t(p) >> 32); }
@@ -456,8 +457,8 @@ __global__ __launch_bounds__(kSmallThreads) void norm_small(const L l, double ma
 }
 
 // ---- Adam ----
-// up: a power of 2 that root, eps and with them the denominator are multiplied by, and size for it, so that an eps near the
-// ends of float32 has a normal reciprocal there (scale_of()).
+// up: a power of 2 that root, eps and with them the denominator are multiplied by, and size for it, so that an eps beyond the
+// ends of float32 counts there, and the quotient of a small one does not overflow before it is multiplied (scale_of()).
 struct Betas { double b1, b2, log_b1, log_b2, eps, up; };
 
 // Counts a tensor's step and turns it into what the update multiplies with, in float64.
@@ -473,23 +474,12 @@ __device__ __forceinline__ Scalars count_step(float *count, double lr, double wd
     return s;
 }
 
-// Root and quotient of the update.  Lists that do not stream take the hardware's own float32 square root and reciprocal, each
-// within a step (2^-23) of its value: 7 instructions for 25, and where one block does the update, or data come from the
-// cache, it waits for them (8e3 values 5.1 us for 6.2, 24e3 4.9 for 5.4).  What is lost is a step of the update, some 1e-3
-// of a step of the parameter.  Beyond the cache memory leaves the time for correctly rounded ones (bfloat16, 268e6 values:
-// 0.93 ms with them, 0.95 without).  The root takes subnormal arguments scaled.
-template <bool kExact> __device__ __forceinline__ float root(float v) {
-    if (kExact) return sqrtf(v);
-    const bool tiny = v < 0x1p-96f;
-    return __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v) * (tiny ? 0x1p-32f : 1.0f);
-}
-template <bool kExact> __device__ __forceinline__ double root(double v) { return sqrt(v); }
-template <bool kExact> __device__ __forceinline__ float quotient(float m, float d) { return kExact ? m / d : m * __builtin_amdgcn_rcpf(d); }
-template <bool kExact> __device__ __forceinline__ double quotient(double m, double d) { return m / d; }
-
 // In float32 (float64 for float64 tensors); the state is float32 or wider, and a 16-bit parameter is rounded once, on
-// its way back.
-template <class C, bool kExact> struct Update {
+// its way back.  Root and quotient are correctly rounded for every list, so that a tensor's new values do not hang on what else is
+// in its list, and hold where the parameter is near 0 and the update is the result.  The hardware's own, each within a step
+// instead of half a one, are 7 instructions for 25; where one block does the update, or data come from the cache, it waits for
+// them (float32, device time: 8e3 values 6.2 us for 5.2, 24e3 5.5 for 5.1, 5e5 6.2 for 5.9, 8e6 40 for 39; nothing beyond the cache).
+template <class C> struct Update {
     C b1, a1, b2, a2, eps, size, scale, keep, l2;
     Factor<C> clip;
     __device__ __forceinline__ C operator()(C x, C g, C &m, C &v) const {
@@ -497,7 +487,7 @@ template <class C, bool kExact> struct Update {
         if (l2 != C(0)) g = fma(l2, x, g);        // not 0 * x, which an infinite x makes NaN
         m = fma(b1, m, a1 * g);
         v = fma(b2, v, a2 * g * g);
-        return fma(-size, quotient<kExact>(m, fma(root<kExact>(v), scale, eps)), x * keep);
+        return fma(-size, m / fma(C(sqrt(v)), scale, eps), x * keep);
     }
 };
 
@@ -509,7 +499,7 @@ __device__ __forceinline__ void piece_adam(E, const L &l, const Piece &q, const 
     T *p = static_cast<T *>(l.template get<1>(q.t)) + q.first;
     const T *g = static_cast<const T *>(l.x(q.t)) + q.first;
     C *m = static_cast<C *>(l.template get<2>(q.t)) + q.first, *v = static_cast<C *>(l.template get<3>(q.t)) + q.first;
-    const Update<C, kStream> f{C(b.b1), C(1.0 - b.b1), C(b.b2), C(1.0 - b.b2), C(b.eps), C(s.size), C(s.root), C(s.keep), C(s.l2), Factor<C>(clip)};
+    const Update<C> f{C(b.b1), C(1.0 - b.b1), C(b.b2), C(1.0 - b.b2), C(b.eps), C(s.size), C(s.root), C(s.keep), C(s.l2), Factor<C>(clip)};
     const int lane = threadIdx.x % kWave, n = q.n;
     auto some = [&](int i, auto count) {        // `count` vectors a lane, all on their way at once
         constexpr int N = count;
@@ -659,8 +649,8 @@ void by_norm(int kind, F &&f) {
     else f(std::integral_constant<int, kNoClip>{});
 }
 
-// The denominator lies between eps and the largest float32 root, 2^64, times its scale, at most 2^27.  The hardware's reciprocal
-// takes a subnormal denominator for 0 and gives 0 where it would be subnormal itself, beyond 2^126: 1 will do in between.
+// A float32 denominator lies between eps and the largest root, 2^64, times its scale, at most 2^27: 2^32 more does not overflow.
+// An eps under float32's subnormal values counts from 2^-181 on.
 double scale_of(double eps) { return eps > 0.0 && eps < 0x1p-126 ? 0x1p32 : eps >= 0x1p64 ? 0x1p-64 : 1.0; }
 
 constexpr int64_t kMaxValues = int64_t(1) << 37;        // of a call: units are counted in 32 bits
