@@ -389,13 +389,14 @@ __global__ __launch_bounds__(kThreads) void norm_finish(const double *part, int 
 // ---- clip ----
 // Multiplies by the clipping factor in the type that the values are computed with: float32 for all but float64 ones, so the
 // factor is rounded (2^-24) and so is the product.  A factor below float32's normal range would lose digits: it is taken in
-// two, the second a power of 2.
+// two, the second a power of 2.  2^-64 keeps the first one normal down to 2^-190; below that 2^-149 does to 2^-275, where a product
+// with the largest value is at most 4 steps of subnormal ones, and the first product cannot overflow (2^-41 2^128).
 template <class C> struct Factor {
     C first, second;
     explicit __device__ __forceinline__ Factor(double c) {
-        const bool tiny = sizeof(C) == 4 && c < 0x1p-126;
-        first = C(tiny ? c * 0x1p64 : c);
-        second = C(tiny ? 0x1p-64 : 1.0);
+        const bool tiny = sizeof(C) == 4 && c < 0x1p-126, least = c < 0x1p-190;
+        first = C(tiny ? c * (least ? 0x1p149 : 0x1p64) : c);
+        second = C(tiny ? (least ? 0x1p-149 : 0x1p-64) : 1.0);
     }
     __device__ __forceinline__ C operator()(C x) const { return x * first * second; }
 };

@@ -1,9 +1,11 @@
 """GPU: results of the optimiser-step operators that are known to the last bit, or by a few roundings, in each of their forms: one
 block, several launches, and lists beyond the cache.  Companions fill a list up to each form without touching what is compared."""
+import math
+
 import numpy as np
 import pytest
 
-from test_gpu_optim import HALF, _t, make
+from test_gpu_optim import HALF, TINY, _t, make
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +61,41 @@ def test_an_update_does_not_hang_on_the_rest_of_the_list(dtype, wd, decoupled):
         results.append(x + m + v)
     for r in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, results[0]))
+
+
+@pytest.mark.parametrize("dtype", ["float64", "float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("more", list(COMPANIONS.values()), ids=list(COMPANIONS))
+@pytest.mark.parametrize("most", [1e-19, 1e-20, 1e-25, 1e-37, 1e-44, 1e-60, 1e-200])
+def test_clipping_by_tiny_factors(dtype, more, most):
+    """Gradients near a type's largest value and a bound far below 1: factors of 1e-57 and less, whose product with them is a normal
+    float32 value.  Factor and product are rounded once each (2 u), to a 16-bit type once more; the last of the steps among
+    subnormal values."""
+    torch, optim = _t()
+    top = {"float64": 1e100, "float16": 6e4}.get(dtype, 3e38)
+    a = torch.tensor([top, -top / 3, top / 1e5, 1.0, 0.0, -2e-4], dtype=torch.float64).to(getattr(torch, dtype)).repeat(700)
+    x = a.cuda()
+    big = torch.full((1,), 1e38, device="cuda")            # the norm is far from 1 whatever the type
+    extra = companion(more, 1)[0]
+    norm = float(optim.clip_grad_norm_([x, big] + extra, most))
+    ref = a.double().numpy()
+    want = math.sqrt(np.sum(ref.astype(np.longdouble) ** 2) + np.longdouble(float(np.float32(1e38))) ** 2)
+    assert abs(norm - want) <= (ref.size + 5) * 2.0 ** -53 * want
+    c = np.longdouble(most) / (np.longdouble(want) + np.longdouble(1e-6))
+    rel = HALF[dtype] + (ref.size + 9) * 2.0 ** -53 + {"float64": 0.0, "float32": 2.0 ** -24}.get(dtype, 2.0 ** -23)
+    err = np.abs(x.double().cpu().numpy() - ref * c) - (1.001 * rel * np.abs(ref * c) + TINY[dtype])
+    assert np.all(err <= 0), (x[:6].tolist(), [float(r) for r in (ref * c)[:6]])
+
+
+@pytest.mark.parametrize("most", [1e-20, 1e-25, 1e-37, 1e-44])
+def test_adam_clips_by_tiny_factors(most):
+    """b1 = 0: the first moment is the clipped gradient, factor and product rounded once each."""
+    torch, optim = _t()
+    g = torch.tensor([3e38, -1e38, 1e33, 1.0], device="cuda")
+    x, m, v, t = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros((), device="cuda")
+    norm = float(optim.adam_step([x], [g], [m], [v], [t], 0.0, betas=(0.0, 0.9), max_norm=most))
+    ref = g.double().cpu().numpy()
+    want = math.sqrt(np.sum(ref ** 2))
+    assert norm == pytest.approx(want, rel=8 * 2.0 ** -53)
+    c = most / (want + 1e-6)
+    got = m.double().cpu().numpy()
+    assert np.all(np.abs(got - ref * c) <= (2.01 * 2.0 ** -24) * np.abs(ref * c) + 2.0 ** -149), (got, ref * c)
