@@ -356,8 +356,10 @@ __global__ __launch_bounds__(kThreads) void norm_partials(const L l, double *par
 
 template <int P> __device__ __forceinline__ double root_of(double acc) { return P == MBRL_NORM_TWO ? sqrt(acc) : acc; }
 
-// What clipping multiplies with.  A norm that is not a number makes it NaN (the comparison is false), an infinite one 0.
+// What clipping multiplies with.  A norm that is not a number makes it NaN (the comparisons are false), an infinite one 0, unless
+// the bound is infinite too: every number is within that.
 __device__ __forceinline__ double factor_of(double norm, double max_norm) {
+    if (max_norm == HUGE_VAL && norm <= max_norm) return 1.0;
     const double c = max_norm / (norm + 1e-6);
     return c > 1.0 ? 1.0 : c;
 }

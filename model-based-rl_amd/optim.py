@@ -49,8 +49,9 @@ def grad_norm(grads, norm_type=2.0):
 
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Multiplies every value of every tensor in `grads` by min(1, max_norm / (norm + 1e-6)), in place, and returns the norm
-    as it was (0-d float64).  A norm within the bound leaves the values untouched, bit for bit.  A NaN norm makes every
-    value NaN, an infinite one makes finite values 0; error_if_nonfinite=True raises RuntimeError before anything is
+    as it was (0-d float64).  A factor of 1 (norm + 1e-6 <= max_norm) leaves the values untouched, bit for bit, and
+    so does max_norm=inf for every norm that is a number.  A NaN norm makes every value NaN, an infinite one makes finite
+    values 0; error_if_nonfinite=True raises RuntimeError before anything is
     changed instead (it waits for the device, so not under graph capture).  Tensors that share memory are refused."""
     b = _bind or bind()
     if error_if_nonfinite:

@@ -99,3 +99,27 @@ def test_adam_clips_by_tiny_factors(most):
     c = most / (want + 1e-6)
     got = m.double().cpu().numpy()
     assert np.all(np.abs(got - ref * c) <= (2.01 * 2.0 ** -24) * np.abs(ref * c) + 2.0 ** -149), (got, ref * c)
+
+
+@pytest.mark.parametrize("more", list(COMPANIONS.values()), ids=list(COMPANIONS))
+@pytest.mark.parametrize("p", [1, 2, math.inf])
+def test_an_infinite_bound_clips_nothing(more, p):
+    """Any norm that is a number is within it, an infinite one too; a NaN norm still makes every value NaN."""
+    torch, optim = _t()
+    for bad in (1.0, math.inf, math.nan):
+        x = make([(300,)], ["float32"], 9)[0]
+        x[7] = bad
+        keep = x.clone()
+        norm = float(optim.clip_grad_norm_([x] + companion(more, 1)[0], math.inf, p))
+        assert math.isnan(norm) if math.isnan(bad) else norm == float(optim.grad_norm([keep], p))
+        assert bool(x.isnan().all()) if math.isnan(bad) else torch.equal(x, keep)
+    states = []
+    for limit in (None, math.inf):
+        g = make([(300,)], ["float32"], 9)[0]
+        g[7] = -math.inf
+        x, m, v, t = torch.ones(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros((), device="cuda")
+        norm = adam([x], [g], [m], [v], [t], more, lr=0.1, max_norm=limit, norm_type=p)
+        assert limit is None or float(norm) == math.inf
+        states.append((x, m, v))
+    for a, b in zip(*states):
+        assert torch.allclose(a, b, rtol=0, atol=0, equal_nan=True) and bool(a[:7].isfinite().all())
