@@ -7,6 +7,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
@@ -87,6 +88,7 @@ struct List {
         const at::Tensor &x = *t[i];
         if (!x.defined() || x.layout() != at::kStrided) bad(i, PyExc_ValueError, "is not a dense (strided) tensor");
         if (x.is_neg()) bad(i, PyExc_ValueError, "is a lazily negated view (resolve_neg() it)");
+        if (x._fw_grad(0).defined()) bad(i, PyExc_ValueError, "has a forward-mode tangent, which these operators do not carry on");
         if (!x.is_non_overlapping_and_dense())
             bad(i, PyExc_ValueError, "has gaps or repeated values between its strides (use .contiguous())");
         if (at.device != x.device() || !x.is_cuda()) at.met(*this, i, x);
@@ -256,7 +258,10 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int kind = norm_code(a[1]);
         Sizes s(g.t.size());
         Place at;
+        const bool recording = c10::GradMode::is_enabled();
         for (size_t i = 0; i < g.t.size(); i++) {
+            if (recording && g.t[i]->requires_grad())
+                g.bad(i, PyExc_ValueError, "requires grad, which the norm does not pass on (call it under torch.no_grad(), or detach())");
             g.check(i, at);
             type_of(g, i, s);
         }

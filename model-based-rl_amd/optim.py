@@ -8,7 +8,8 @@ does not.  `strategies.VariationalOptimization.optimize` calls these under SOLVE
 
 All functions take lists of float64 / float32 / bfloat16 / float16 tensors of one GPU (types may be mixed), launch on the
 current stream, never wait for the device (but for error_if_nonfinite) and can be captured into a graph.  Tensors have to be
-dense -- any order of dimensions, any alignment, no gaps or repeats.  There is no CPU path.
+dense -- any order of dimensions, any alignment, no gaps or repeats.  There is no CPU path.  Autograd records none of them:
+what is changed in place is changed as under torch.no_grad(), and forward-mode tangents are refused.
 """
 import ctypes as C
 import importlib.util
@@ -42,7 +43,8 @@ def bind():
 
 def grad_norm(grads, norm_type=2.0):
     """Norm over all values of all tensors in `grads` as a 0-d float64 tensor, summed in float64.  norm_type 1, 2 or inf.
-    0 for an empty list, NaN if any value is NaN.  The same values in tensors of the same sizes give the same bits wherever
+    0 for an empty list, NaN if any value is NaN.  The result carries no gradient: tensors that require grad are refused unless
+    under torch.no_grad().  The same values in tensors of the same sizes give the same bits wherever
     they lie, so ranks that hold the same gradients find the same norm."""
     return (_bind or bind()).grad_norm(grads, norm_type)
 
@@ -58,7 +60,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
         grads = grads if isinstance(grads, torch.Tensor) else tuple(grads)        # an iterator would be empty the second time
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise ValueError("clip_grad_norm_: error_if_nonfinite waits for the device and cannot be captured into a graph")
-        norm = float(b.grad_norm(grads, norm_type))
+        with torch.no_grad():
+            norm = float(b.grad_norm(grads, norm_type))
         if not math.isfinite(norm):
             raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % norm)
     return b.clip_grad_norm_(grads, max_norm, norm_type)
