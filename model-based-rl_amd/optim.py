@@ -82,7 +82,8 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.999
 
 class FusedAdam(torch.optim.Optimizer):
     """torch.optim.Adam's rule as one adam_step over all parameters that have a gradient, with the gradients clipped by their
-    global norm on the way (max_norm; None: not).  `grad_norm` holds the norm of the last step (0-d float64) then.
+    global norm on the way (max_norm; None: not).  `grad_norm` holds the norm of the last step (0-d float64; 0 of a step without
+    gradients) then, else None.
 
     lr and weight_decay go by parameter group; betas, eps and decoupled_weight_decay are the same for all groups.  State is
     named and shaped as torch.optim.Adam's (float32 moments for 16-bit parameters), so a state_dict of either loads
@@ -149,6 +150,11 @@ class FusedAdam(torch.optim.Optimizer):
         if params:
             self.grad_norm = adam_step(params, grads, avgs, sqs, steps, lr, first["betas"], first["eps"], wd,
                                        first["decoupled_weight_decay"], self.max_norm, self.norm_type)
+        elif self.max_norm is None:
+            self.grad_norm = None
+        else:        # of no gradients, as clip_grad_norm_([])
+            device = next((p.device for group in self.param_groups for p in group["params"]), None)
+            self.grad_norm = torch.zeros((), dtype=torch.float64, device=device)
         return loss
 
     def __getstate__(self):        # for copies and pickles; the base class keeps its own three attributes only

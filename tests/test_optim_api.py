@@ -40,3 +40,25 @@ def test_tangents_are_refused():
                     call()
     with pytest.raises(lib.MbrlError, match="no CPU path"):
         optim.grad_norm([torch.ones(4)])
+
+
+def test_the_norm_of_a_step_without_gradients(monkeypatch):
+    """Not the norm of an earlier step."""
+    p = torch.nn.Parameter(Z(3))
+    monkeypatch.setattr(optim, "adam_step", lambda *a: None if a[10] is None else torch.tensor(5.0, dtype=torch.float64))
+    opt = optim.FusedAdam([p], 0.1, max_norm=1.0)
+    opt.step()
+    assert float(opt.grad_norm) == 0.0 and opt.grad_norm.dtype == torch.float64 and opt.grad_norm.shape == ()
+    p.grad = torch.ones(3)
+    opt.step()
+    assert float(opt.grad_norm) == 5.0
+    opt.zero_grad()
+    opt.step()
+    assert float(opt.grad_norm) == 0.0
+    p.grad, opt.max_norm = torch.ones(3), None
+    opt.step()
+    assert opt.grad_norm is None
+    opt.grad_norm = torch.tensor(5.0)
+    opt.zero_grad()
+    opt.step()
+    assert opt.grad_norm is None
