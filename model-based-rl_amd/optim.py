@@ -161,20 +161,35 @@ class FusedAdam(torch.optim.Optimizer):
         return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type, grad_norm=None)
 
     def load_state_dict(self, state_dict):
-        """As Optimizer.load_state_dict, but moments keep their float32 (or float64) values: the base class rounds them to
-        their parameter's type."""
-        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]) or \
-                any("max_exp_avg_sq" in s for s in state_dict["state"].values()):
-            raise ValueError("FusedAdam: amsgrad and maximize are not offered")
-        super().load_state_dict(state_dict)
-        for g in self.param_groups:
-            g.setdefault("decoupled_weight_decay", self.defaults["decoupled_weight_decay"])
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            saved = state_dict["state"].get(i)
-            if not saved or "exp_avg" not in saved:
-                continue
-            s = self._new_state(p)
-            s["step"].copy_(torch.as_tensor(saved["step"], dtype=torch.float32))
-            for k in ("exp_avg", "exp_avg_sq"):
-                s[k].copy_(saved[k])
+        """As Optimizer.load_state_dict, its hooks too, but moments keep their float32 (or float64) values: the base class
+        rounds them to their parameter's type."""
+        ids, loaded = [], {}
+
+        def before(_, state_dict):        # last of its kind: sees what the other hooks made of the dict
+            if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]) or \
+                    any("max_exp_avg_sq" in s for s in state_dict["state"].values()):
+                raise ValueError("FusedAdam: amsgrad and maximize are not offered")
+            ids.extend(i for g in state_dict["param_groups"] for i in g["params"])
+            for i in ids:
+                saved = state_dict["state"].get(i)
+                if not saved or "exp_avg" not in saved:
+                    continue
+                loaded[i] = saved
+
+        def after(_):                     # first of its kind: the others see the moments as they stay
+            for g in self.param_groups:
+                g.setdefault("decoupled_weight_decay", self.defaults["decoupled_weight_decay"])
+            for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+                if i not in loaded:
+                    continue
+                s = self._new_state(p)
+                s["step"].copy_(torch.as_tensor(loaded[i]["step"], dtype=torch.float32))
+                for k in ("exp_avg", "exp_avg_sq"):
+                    s[k].copy_(loaded[i][k])
+
+        hooks = [self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()

@@ -62,3 +62,41 @@ def test_the_norm_of_a_step_without_gradients(monkeypatch):
     opt.zero_grad()
     opt.step()
     assert opt.grad_norm is None
+
+
+def _state(p, value):
+    return {"step": torch.tensor(7.0), "exp_avg": torch.full_like(p, value, dtype=torch.float32),
+            "exp_avg_sq": torch.full_like(p, value * value, dtype=torch.float32)}
+
+
+def test_hooks_of_loading_count():
+    """What a hook makes of the dict is what is loaded, and a hook behind sees, and may change, what stays."""
+    p = torch.nn.Parameter(Z(4, dtype=torch.bfloat16))
+    opt = optim.FusedAdam([p], 0.1)
+    saved = {"state": {0: _state(p, 0.1)}, "param_groups": opt.state_dict()["param_groups"]}
+
+    def other_moments(_, sd):
+        return dict(sd, state={0: _state(p, 0.3)})
+    seen = []
+
+    def behind(o):
+        seen.append(o.state[p]["exp_avg"].clone())
+        o.state[p]["exp_avg_sq"].fill_(2.0)
+    handles = [opt.register_load_state_dict_pre_hook(other_moments), opt.register_load_state_dict_post_hook(behind)]
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        want = torch.full((4,), 0.3)
+        assert seen[-1].dtype == torch.float32 and torch.equal(seen[-1], want) and torch.equal(opt.state[p]["exp_avg"], want)
+        assert bool((opt.state[p]["exp_avg_sq"] == 2.0).all())
+    for h in handles:
+        h.remove()
+    opt.load_state_dict(saved)
+    assert torch.equal(opt.state[p]["exp_avg"], torch.full((4,), 0.1)) and len(seen) == 2
+
+    def plain(_, sd):        # a hook may take out what is not offered
+        return dict(sd, param_groups=[dict(g, amsgrad=False) for g in sd["param_groups"]])
+    ams = dict(saved, param_groups=[dict(g, amsgrad=True) for g in saved["param_groups"]])
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(ams)
+    opt.register_load_state_dict_pre_hook(plain)
+    opt.load_state_dict(ams)
