@@ -162,7 +162,8 @@ class FusedAdam(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As Optimizer.load_state_dict, its hooks too, but moments keep their float32 (or float64) values: the base class
-        rounds them to their parameter's type."""
+        rounds them to their parameter's type.  Moments of another shape than their parameter are refused before
+        anything is changed."""
         ids, loaded = [], {}
 
         def before(_, state_dict):        # last of its kind: sees what the other hooks made of the dict
@@ -170,10 +171,13 @@ class FusedAdam(torch.optim.Optimizer):
                     any("max_exp_avg_sq" in s for s in state_dict["state"].values()):
                 raise ValueError("FusedAdam: amsgrad and maximize are not offered")
             ids.extend(i for g in state_dict["param_groups"] for i in g["params"])
-            for i in ids:
+            for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
                 saved = state_dict["state"].get(i)
                 if not saved or "exp_avg" not in saved:
                     continue
+                for k in ("exp_avg", "exp_avg_sq"):
+                    if saved[k].shape != p.shape:
+                        raise ValueError("FusedAdam: %s of parameter %r has another shape than it" % (k, i))
                 loaded[i] = saved
 
         def after(_):                     # first of its kind: the others see the moments as they stay

@@ -100,3 +100,17 @@ def test_hooks_of_loading_count():
         opt.load_state_dict(ams)
     opt.register_load_state_dict_pre_hook(plain)
     opt.load_state_dict(ams)
+
+
+def test_moments_of_another_shape_are_refused():
+    p = torch.nn.Parameter(Z(4, 6))
+    opt = optim.FusedAdam([p], 0.1)
+    opt.load_state_dict({"state": {0: _state(p, 0.1)}, "param_groups": opt.state_dict()["param_groups"]})
+    for shape in ((6,), (1,), (4, 1), (24,), (1, 4, 6)):
+        wrong = {"state": {0: _state(Z(shape), 0.2)}, "param_groups": opt.state_dict()["param_groups"]}
+        wrong["param_groups"][0]["lr"] = 9.0
+        with pytest.raises(ValueError, match="another shape"):
+            opt.load_state_dict(wrong)
+        assert opt.param_groups[0]["lr"] == 0.1 and torch.equal(opt.state[p]["exp_avg"], torch.full((4, 6), 0.1))
+    with pytest.raises(ValueError):                    # as the base class: another number of parameters
+        opt.load_state_dict({"state": {}, "param_groups": [dict(opt.state_dict()["param_groups"][0], params=[0, 1])]})
