@@ -106,6 +106,15 @@ class FusedAdam(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       decoupled_weight_decay=bool(decoupled_weight_decay)))
 
+    def add_param_group(self, param_group):
+        for k in ("amsgrad", "maximize"):
+            if param_group.get(k):
+                raise ValueError("FusedAdam: %s is not offered" % k)
+        for k in ("max_norm", "norm_type"):
+            if k in param_group:
+                raise ValueError("FusedAdam: %s is the optimiser's, not a parameter group's" % k)
+        super().add_param_group(param_group)
+
     def _common(self):
         first = self.param_groups[0]
         for g in self.param_groups:

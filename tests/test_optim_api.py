@@ -114,3 +114,16 @@ def test_moments_of_another_shape_are_refused():
         assert opt.param_groups[0]["lr"] == 0.1 and torch.equal(opt.state[p]["exp_avg"], torch.full((4, 6), 0.1))
     with pytest.raises(ValueError):                    # as the base class: another number of parameters
         opt.load_state_dict({"state": {}, "param_groups": [dict(opt.state_dict()["param_groups"][0], params=[0, 1])]})
+
+
+@pytest.mark.parametrize("key,value", [("maximize", True), ("amsgrad", True), ("max_norm", 1.0), ("norm_type", 1)])
+def test_groups_with_options_that_would_not_be_followed(key, value):
+    """A group that asks to maximise must not be minimised."""
+    p, q = torch.nn.Parameter(Z(2)), torch.nn.Parameter(Z(2))
+    with pytest.raises(ValueError, match=key):
+        optim.FusedAdam([{"params": [p], key: value}], 0.1)
+    opt = optim.FusedAdam([p], 0.1)
+    with pytest.raises(ValueError, match=key):
+        opt.add_param_group({"params": [q], key: value})
+    opt.add_param_group({"params": [q], "amsgrad": False, "maximize": False, "name": "second"})
+    assert len(opt.param_groups) == 2
