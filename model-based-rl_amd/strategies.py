@@ -274,7 +274,9 @@ class VariationalOptimization(nn.Module):
         if grad_sync is not None:
             grad_sync(grads)
         max_norm, norm = float(self.cfg.SOLVER.CLIP_GRAD_NORM), None
-        if max_norm and not self.cfg.SOLVER.FUSED:
+        if self.cfg.SOLVER.FUSED and isinstance(self.optimizer, optim.FusedAdam):        # clips on its way, by the bound as it is now
+            self.optimizer.max_norm = max_norm or None
+        elif max_norm:
             norm = optim.clip_grad_norm_(grads, max_norm)
         if self.cfg.SOLVER.OPTIMIZER == "sgd":
             nn.utils.clip_grad_value_(self.parameters(), 1)

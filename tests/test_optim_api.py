@@ -127,3 +127,27 @@ def test_groups_with_options_that_would_not_be_followed(key, value):
         opt.add_param_group({"params": [q], key: value})
     opt.add_param_group({"params": [q], "amsgrad": False, "maximize": False, "name": "second"})
     assert len(opt.param_groups) == 2
+
+
+def test_the_strategy_clips_by_the_bound_of_the_moment(monkeypatch):
+    """SOLVER.CLIP_GRAD_NORM is read at every step, whichever optimiser follows it."""
+    from mbrl_amd.strategies import VariationalOptimization
+    from test_strategy_host import cfg_vo, fake_agent
+    bounds = []
+
+    def adam_step(*a):
+        bounds.append(a[10])
+        return None if a[10] is None else torch.sqrt(sum(g.double().square().sum() for g in a[1]))
+    monkeypatch.setattr(optim, "adam_step", adam_step)
+    cfg = cfg_vo()
+    cfg.SOLVER.FUSED = True
+    pol = VariationalOptimization(cfg, fake_agent())
+    loss = lambda: (pol.mean.sum() * 3.0).expand(4, 5) + 0 * pol.sd.sum()      # noqa: E731
+    for bound in (0.0, 2.5, 0.5, 0.0):
+        cfg.SOLVER.CLIP_GRAD_NORM = bound
+        stats = pol.optimize(loss())
+        assert bounds[-1] == (bound or None)
+        if bound:        # of every entry of the mean 3 over 5 steps, 5 entries
+            assert stats["grad_norm"] == pytest.approx(15.0 * 5 ** 0.5)
+        else:
+            assert "grad_norm" not in stats
