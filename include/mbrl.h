@@ -216,8 +216,9 @@ int mbrl_lane_map(int nq, int nv, int nu, int fd_mode, int *units_per_pair, int 
  * arbitrary before and after; one per call in flight (calls on the same stream may share one, captured graphs that can run
  * at the same time must not).  All launches go to the
  * calling thread's current HIP device, which must own the memory and the stream; no call waits for the device, and all can
- * be captured into a HIP graph.  Results depend on the values, sizes and types alone, not on timing or addresses: no atomics,
- * every sum in a fixed order. */
+ * be captured into a HIP graph.  Results depend on the operator, the values, sizes and types alone, not on timing or
+ * addresses: no atomics, every sum in a fixed order.  The three operators order the sum of a norm each in their own way, so
+ * their norms of one list may differ in the last bits. */
 #define MBRL_DT_DOUBLE 0
 #define MBRL_DT_FLOAT 1
 #define MBRL_DT_BFLOAT 2
@@ -247,7 +248,9 @@ int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel,
  *     param = param * (decoupled ? 1 - lr[i] weight_decay[i] : 1) - lr[i] / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps).
  * exp_avgs (m) and exp_avg_sqs (v) are fp64 for fp64 parameters and fp32 for all others; gradients have their parameter's
  * type and are left as they are.  Arithmetic in the moments' type, one rounding to a 16-bit parameter.  steps[i]: one
- * fp32 value in device memory for each tensor, empty ones too (exact up to 2^24 steps).  norm != NULL: the norm over all gradients is left there (device).
+ * fp32 value in device memory for each tensor, empty ones too (exact up to 2^24 steps).  A 16-bit gradient is not rounded
+ * between clipping and the update.  Root and quotient are correctly rounded.  An eps below 2^-181 counts as 0 for fp32
+ * moments.  norm != NULL: the norm over all gradients is left there (device).
  * Memory that is written and shared with another tensor of the call is refused (-7). */
 int mbrl_adam_step(int64_t count, void *const *params, const void *const *grads, void *const *exp_avgs,
                    void *const *exp_avg_sqs, float *const *steps, const int64_t *numel, const int *dtype, const double *lr,

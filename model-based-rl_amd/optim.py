@@ -45,7 +45,8 @@ def grad_norm(grads, norm_type=2.0):
     """Norm over all values of all tensors in `grads` as a 0-d float64 tensor, summed in float64.  norm_type 1, 2 or inf.
     0 for an empty list, NaN if any value is NaN.  The result carries no gradient: tensors that require grad are refused unless
     under torch.no_grad().  The same values in tensors of the same sizes give the same bits wherever
-    they lie, so ranks that hold the same gradients find the same norm."""
+    they lie, so ranks that hold the same gradients find the same norm; the other operators order the sum in their own way, and
+    their norms may differ from this one in the last bits."""
     return (_bind or bind()).grad_norm(grads, norm_type)
 
 
@@ -53,8 +54,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Multiplies every value of every tensor in `grads` by min(1, max_norm / (norm + 1e-6)), in place, and returns the norm
     as it was (0-d float64).  A factor of 1 (norm + 1e-6 <= max_norm) leaves the values untouched, bit for bit, and
     so does max_norm=inf for every norm that is a number.  A NaN norm makes every value NaN, an infinite one makes finite
-    values 0; error_if_nonfinite=True raises RuntimeError before anything is
-    changed instead (it waits for the device, so not under graph capture).  Tensors that share memory are refused."""
+    values 0; error_if_nonfinite=True raises RuntimeError before anything is changed instead (it takes the norm once more and
+    waits for the device, so not under graph capture).  Tensors that share memory are refused."""
     b = _bind or bind()
     if error_if_nonfinite:
         grads = grads if isinstance(grads, torch.Tensor) else tuple(grads)        # an iterator would be empty the second time
@@ -74,7 +75,8 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas=(0.9, 0.999
     exp_avgs / exp_avg_sqs: float64 for float64 parameters, float32 for all others, shaped and laid out like their
     parameter; steps: one float32 value in device memory each, counted up here; lr, weight_decay: one number or one for
     each tensor; decoupled: weight decay on the parameter (AdamW) instead of on the gradient.  max_norm: the gradients enter
-    as clip_grad_norm_ would leave them, but are not written; returns their norm (0-d float64) then, else None.
+    multiplied as by clip_grad_norm_, but are not written, and 16-bit ones not rounded in between; returns their norm
+    (0-d float64) then, else None.
     Memory that is written must not be shared between tensors."""
     return (_bind or bind()).adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay,
                                        decoupled, max_norm, norm_type)
