@@ -23,7 +23,7 @@
 //   8e6       6.6 us, 4.9 TB/s   14.7 us, 6.5 TB/s   40 us, 5.6 TB/s     46 us          from the cache
 //   268e6     164 us, 6.5 TB/s   525 us, 6.1 TB/s    1.22 ms, 6.2 TB/s   1.37 ms        from memory
 // (clip: two reads and a write).  Below that it is the launches: an empty one takes 2.2 us of the device and 3.7 us of the
-// host, so small lists are done in one (a call of 2 or 10 tensors: 4.3 us of the host for a norm).
+// host, so small lists are done in one.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
