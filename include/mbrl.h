@@ -238,7 +238,8 @@ int mbrl_grad_norm(int64_t count, const void *const *grads, const int64_t *numel
 
 /* The same, then every value is multiplied by min(1, max_norm / (norm + 1e-6)) in place (in fp64 for fp64, else in
  * fp32, rounded once to a 16-bit type).  A NaN norm makes every value NaN, an infinite one makes finite values 0 and infinite ones NaN.
- * max_norm >= 0; an infinite one leaves all values as they are, an infinite norm too (but NaN for a NaN norm).  Tensors that share memory are refused (-7). */
+ * max_norm >= 0; an infinite one leaves all values as they are whatever the norm, but for a NaN norm.  Tensors that share
+ * memory are refused (-7). */
 int mbrl_clip_grad_norm(int64_t count, void *const *grads, const int64_t *numel, const int *dtype, int norm_type,
                         double max_norm, void *workspace, int64_t workspace_bytes, double *norm, void *hip_stream);
 

@@ -44,9 +44,9 @@ def bind():
 def grad_norm(grads, norm_type=2.0):
     """Norm over all values of all tensors in `grads` as a 0-d float64 tensor, summed in float64.  norm_type 1, 2 or inf.
     0 for an empty list, NaN if any value is NaN.  The result carries no gradient: tensors that require grad are refused unless
-    under torch.no_grad().  The same values in tensors of the same sizes give the same bits wherever
-    they lie, so ranks that hold the same gradients find the same norm; the other operators order the sum in their own way, and
-    their norms may differ from this one in the last bits."""
+    under torch.no_grad().  The same values in tensors of the same sizes give the same bits wherever they lie, so ranks that
+    hold the same gradients find the same norm; the other operators order the sum in their own way, and their norms may
+    differ from this one in the last bits."""
     return (_bind or bind()).grad_norm(grads, norm_type)
 
 
@@ -109,11 +109,12 @@ class FusedAdam(torch.optim.Optimizer):
                                       decoupled_weight_decay=bool(decoupled_weight_decay)))
 
     def add_param_group(self, param_group):
+        keys = param_group if isinstance(param_group, dict) else {}        # the base class refuses what is no dict
         for k in ("amsgrad", "maximize"):
-            if param_group.get(k):
+            if keys.get(k):
                 raise ValueError("FusedAdam: %s is not offered" % k)
         for k in ("max_norm", "norm_type"):
-            if k in param_group:
+            if k in keys:
                 raise ValueError("FusedAdam: %s is the optimiser's, not a parameter group's" % k)
         super().add_param_group(param_group)
 

@@ -125,6 +125,8 @@ def test_groups_with_options_that_would_not_be_followed(key, value):
     opt = optim.FusedAdam([p], 0.1)
     with pytest.raises(ValueError, match=key):
         opt.add_param_group({"params": [q], key: value})
+    with pytest.raises(TypeError):
+        opt.add_param_group([q])                       # as the base class
     opt.add_param_group({"params": [q], "amsgrad": False, "maximize": False, "name": "second"})
     assert len(opt.param_groups) == 2
 
