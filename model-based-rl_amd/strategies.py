@@ -264,7 +264,8 @@ class VariationalOptimization(nn.Module):
         baselines of PR / IR / SIR are then per-shard statistics.
         SOLVER.CLIP_GRAD_NORM > 0 bounds the global norm of the (summed) gradient before the step -- differences through
         contacts grow with the horizon -- and adds it, as it was before clipping, to the returned statistics.  The bound is
-        read here, at every step, for torch's optimisers and the fused one.  Every rank finds the same norm for the same summed gradient, so the ranks' parameters stay the same."""
+        read here, at every step, for torch's optimisers and the fused one.  Every rank finds the same norm for the same
+        summed gradient, so the ranks' parameters stay the same."""
         loss, stats = self.loss_functions.get(self.method, self.R_loss)(batch_loss)
         if self.local_batch != self.batch_size:
             loss = loss * (float(self.local_batch) / float(self.batch_size))
